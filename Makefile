@@ -22,7 +22,11 @@ ifdef SANITIZE
 CXXFLAGS += -fsanitize=$(SANITIZE) -fno-omit-frame-pointer
 LDFLAGS_EXTRA := -fsanitize=$(SANITIZE)
 endif
-HIPCCFLAGS := -O3 -std=c++17 -fPIC -MMD -MP --offload-arch=gfx950 -Icsrc
+# -packed-fp32-ops: some packed fp32 forms that the compiler makes of plain
+# float code give wrong results on this platform (the host pass warns that
+# it does not know the feature).
+HIPCCFLAGS := -O3 -std=c++17 -fPIC -MMD -MP --offload-arch=gfx950 -Icsrc \
+  -Xclang -target-feature -Xclang -packed-fp32-ops
 
 CC_SRCS := $(shell find csrc -name '*.cc' ! -path 'csrc/bindings/*' ! -path 'csrc/bench/*')
 HIP_SRCS := $(shell find csrc -name '*.hip' 2>/dev/null)
