@@ -11,6 +11,7 @@
 #include <pybind11/stl.h>
 
 #include "algorithms/factory.h"
+#include "bindings/experts.h"
 #include "collectives/collectives.h"
 #include "collectives/schedule.h"
 #include "collectives/reduce_fns.h"
@@ -1109,4 +1110,6 @@ PYBIND11_MODULE(_C, m) {
           py::arg("bytes"),
           py::arg("stream") = 0)
       .def("debug_flags", &hip::HipBroadcastOneToAll::debugFlags);
+
+  bindExperts(m);
 }

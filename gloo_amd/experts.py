@@ -1,0 +1,495 @@
+"""Operators of expert-parallel layers, on either side of an alltoallv.
+
+    weights, ids = route(logits, k)           # which experts, how much
+    p = plan(ids, num_experts)                # token copies, by expert
+    rows = pack(x, p)                         # the alltoallv's send buffer
+    ...                                       # the experts
+    out = combine(rows, p, weights)           # back to tokens
+
+`pack_fp8` packs in 8 bits with a scale for each block of 128 instead, and
+`fp8_matmul` multiplies such rows by their experts' weights; `ExpertExchange`
+runs the whole way over a process group. All operators are hand-written HIP
+kernels (csrc/hip/experts.hip, csrc/hip/fp8.hip) that run asynchronously on
+the current stream of their tensors' device, allocate with torch's allocator
+and may be captured into a graph. Tensors have to be on a GPU; wrong arguments
+raise ValueError before anything is launched.
+
+8-bit values are torch.float8_e4m3fn. Their scales are powers of two
+(torch.float8_e8m0fnu): the least that brings a block's largest value to 448
+or less, 2^-127 at least, 2^0 for a block of zeros and NaN for one that holds
+inf or NaN.
+"""
+from typing import NamedTuple, Optional
+
+import torch
+import torch.distributed as dist
+from torch.autograd.function import once_differentiable
+
+import gloo_amd as ga
+
+_C = ga._C
+
+FP8 = torch.float8_e4m3fn
+FP8_SCALE = torch.float8_e8m0fnu
+FP8_BLOCK = 128
+_FLOATS = {torch.float32: ga.DType.f32, torch.float16: ga.DType.f16,
+           torch.bfloat16: ga.DType.bf16}
+
+
+class ExpertPlan(NamedTuple):
+    """Token copies sorted by expert, in order of tokens within one.
+
+    position [tokens, k] int32: a copy's row. A copy for no expert stands
+        behind all others, and its row r is told as ~r, a negative number.
+    counts [experts] int32: copies of each expert.
+    offsets [experts + 1] int32: where each expert's rows begin; the last
+        one is the number of copies that have an expert.
+    """
+    position: torch.Tensor
+    counts: torch.Tensor
+    offsets: torch.Tensor
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _tensor(t, name, dim, dtypes, like=None):
+    _need(isinstance(t, torch.Tensor), f"{name}: a tensor is needed")
+    _need(t.dim() == dim, f"{name}: {dim} dimensions are needed, got "
+          f"{tuple(t.shape)}")
+    _need(t.dtype in dtypes, f"{name}: one of {[str(d) for d in dtypes]} is "
+          f"needed, got {t.dtype}")
+    _need(like is None or t.device == like.device,
+          f"{name}: is on {t.device}, and others are on "
+          f"{like.device if like is not None else None}")
+
+
+def _gpu(t, name):
+    """The last check before a launch: the others hold on any device."""
+    _need(t.is_cuda, f"{name}: tensors on a GPU are needed, got {t.device}")
+
+
+def _stream(t):
+    return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def _adjacent(t):
+    """t, or a copy of it, with adjacent elements in its last dimension."""
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+
+
+def _blocks(n):
+    return (n + FP8_BLOCK - 1) // FP8_BLOCK
+
+
+# ------------------------------------------------------------------- router
+
+
+class _Route(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, bias, k, score, groups, topk_groups,
+                group_score, renormalize, scale):
+        tokens, experts = logits.shape
+        x = _adjacent(logits.detach())
+        weights = torch.empty(tokens, k, dtype=torch.float32,
+                              device=x.device)
+        ids = torch.empty(tokens, k, dtype=torch.int32, device=x.device)
+        _C.hip_expert_route(
+            x.data_ptr(), x.stride(0), _FLOATS[x.dtype],
+            0 if bias is None else bias.data_ptr(), tokens, experts, k,
+            score, groups, topk_groups, group_score, renormalize, scale,
+            weights.data_ptr(), ids.data_ptr(), x.get_device(), _stream(x))
+        ctx.mark_non_differentiable(ids)
+        ctx.save_for_backward(logits, ids)
+        ctx.options = (score, renormalize, scale)
+        return weights, ids
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad, _):
+        logits, ids = ctx.saved_tensors
+        score, renormalize, scale = ctx.options
+        x = _adjacent(logits.detach())
+        grad = grad.contiguous()
+        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        _C.hip_expert_route_backward(
+            x.data_ptr(), x.stride(0), _FLOATS[x.dtype], x.shape[0],
+            x.shape[1], ids.shape[1], score, renormalize, scale,
+            ids.data_ptr(), grad.data_ptr(), dx.data_ptr(), x.get_device(),
+            _stream(x))
+        return (dx,) + (None,) * 8
+
+
+def route(logits, k, *, score="softmax", bias=None, groups=1, topk_groups=1,
+          group_score="max", renormalize=True, scale=1.0):
+    """The k experts of each token and their weights.
+
+    logits [tokens, experts] in float32, float16 or bfloat16. Scores are
+    their softmax or sigmoid. The k experts with the largest score + bias
+    (bias [experts] float32; without one, with the largest logits) are
+    chosen, ties go to the lower number, and they are listed from the best
+    on. With groups > 1 the experts are parted into groups of adjacent ones,
+    and only those of the topk_groups best groups can be chosen; a group is
+    as good as its best expert ("max") or as its two best ones' sum
+    ("top2"). The bias takes part in the choice only: a chosen expert's
+    weight is its score, divided by the sum of the chosen ones' where
+    `renormalize` is set, times `scale`.
+
+    An expert whose logit is -inf or NaN is never chosen: where a token has
+    fewer experts than k, the others are -1, with weight 0. +inf counts as
+    the largest float32.
+
+    Returns (weights [tokens, k] float32, experts [tokens, k] int32). The
+    weights are differentiable with respect to the logits.
+    """
+    _tensor(logits, "logits", 2, _FLOATS)
+    tokens, experts = logits.shape
+    _need(1 <= experts <= _C.MAX_EXPERTS,
+          f"route: 1 to {_C.MAX_EXPERTS} experts, got {experts}")
+    _need(1 <= k <= min(experts, _C.MAX_TOPK),
+          f"route: k is 1 to {min(experts, _C.MAX_TOPK)} here, got {k}")
+    _need(score in ("softmax", "sigmoid"),
+          f"route: score is 'softmax' or 'sigmoid', got {score!r}")
+    _need(group_score in ("max", "top2"),
+          f"route: group_score is 'max' or 'top2', got {group_score!r}")
+    _need(1 <= groups <= _C.MAX_EXPERT_GROUPS and experts % groups == 0,
+          f"route: {experts} experts in {groups} equal groups (at most "
+          f"{_C.MAX_EXPERT_GROUPS})")
+    _need(1 <= topk_groups <= groups,
+          f"route: topk_groups is 1 to {groups}, got {topk_groups}")
+    _need(groups == 1 or k <= topk_groups * (experts // groups),
+          f"route: {topk_groups} groups of {experts // groups} experts hold "
+          f"fewer than k = {k}")
+    if bias is not None:
+        _tensor(bias, "bias", 1, (torch.float32,), logits)
+        _need(bias.shape[0] == experts,
+              f"bias: {experts} values are needed, got {bias.shape[0]}")
+        bias = bias.detach().contiguous()
+    _gpu(logits, "route")
+    return _Route.apply(logits, bias, k, score, groups, topk_groups,
+                        group_score, bool(renormalize), float(scale))
+
+
+# ------------------------------------------------- plan, pack and combine
+
+
+def plan(experts, num_experts):
+    """Sorts token copies by expert (stable). experts [tokens, k] int32, as
+    `route` gives them; numbers outside [0, num_experts) are no expert."""
+    _tensor(experts, "experts", 2, (torch.int32,))
+    _need(1 <= num_experts <= _C.MAX_EXPERTS,
+          f"plan: 1 to {_C.MAX_EXPERTS} experts, got {num_experts}")
+    ids = experts.contiguous()
+    n = ids.numel()
+    _need(n < 2 ** 31, f"plan: fewer than 2^31 token copies, got {n}")
+    _gpu(ids, "plan")
+    dev = ids.device
+    position = torch.empty(ids.shape, dtype=torch.int32, device=dev)
+    # one allocation: the counts, then the offsets on a border of 16 bytes
+    start = (num_experts + 3) // 4 * 4
+    both = torch.empty(start + num_experts + 1, dtype=torch.int32,
+                       device=dev)
+    counts, offsets = both[:num_experts], both[start:]
+    size = _C.hip_expert_plan_workspace(n, num_experts)
+    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+    _C.hip_expert_plan(
+        ids.data_ptr(), n, num_experts, position.data_ptr(),
+        counts.data_ptr(), offsets.data_ptr(),
+        work.data_ptr() if size else 0, size, ids.get_device(), _stream(ids))
+    return ExpertPlan(position, counts, offsets)
+
+
+def _rows_args(position, hidden, dtype):
+    return (position.data_ptr(), position.shape[0], position.shape[1],
+            hidden, _FLOATS[dtype])
+
+
+def _check_plan(p, tokens, like):
+    position = p.position
+    _tensor(position, "plan.position", 2, (torch.int32,), like)
+    _need(position.is_contiguous(), "plan.position has to be contiguous")
+    _need(tokens is None or position.shape[0] == tokens,
+          f"the plan is for {position.shape[0]} tokens, got {tokens}")
+    _need(position.shape[1] > 0 and position.numel() < 2 ** 31,
+          f"plan.position: got {tuple(position.shape)}")
+    return position
+
+
+def _pack(x, position):
+    x = _adjacent(x)
+    hidden = x.shape[1]
+    rows = torch.empty(position.numel(), hidden, dtype=x.dtype,
+                       device=x.device)
+    if rows.numel():
+        _C.hip_expert_pack(
+            *_rows_args(position, hidden, x.dtype), x.data_ptr(),
+            x.stride(0), rows.data_ptr(), x.get_device(), _stream(x))
+    return rows
+
+
+def _combine(rows, position, weights):
+    rows = _adjacent(rows)
+    hidden = rows.shape[1]
+    out = torch.empty(position.shape[0], hidden, dtype=rows.dtype,
+                      device=rows.device)
+    if out.numel():
+        _C.hip_expert_combine(
+            *_rows_args(position, hidden, rows.dtype), rows.data_ptr(),
+            rows.stride(0), 0 if weights is None else weights.data_ptr(),
+            out.data_ptr(), rows.get_device(), _stream(rows))
+    return out
+
+
+class _Pack(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, position):
+        ctx.save_for_backward(position)
+        return _pack(x.detach(), position)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        position, = ctx.saved_tensors
+        return _combine(grad, position, None), None
+
+
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, rows, position, weights):
+        ctx.save_for_backward(rows, position, weights)
+        return _combine(rows.detach(), position, weights)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad):
+        rows, position, weights = ctx.saved_tensors
+        if weights is None:
+            return _pack(grad, position), None, None
+        rows, grad = _adjacent(rows.detach()), _adjacent(grad)
+        drows = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
+        dw = torch.empty(weights.shape, dtype=torch.float32,
+                         device=rows.device)
+        if drows.numel():
+            _C.hip_expert_combine_backward(
+                *_rows_args(position, rows.shape[1], rows.dtype),
+                rows.data_ptr(), rows.stride(0), weights.data_ptr(),
+                grad.data_ptr(), grad.stride(0), drows.data_ptr(),
+                dw.data_ptr(), rows.get_device(), _stream(rows))
+        else:
+            dw.zero_()
+        return drows, None, dw
+
+
+def pack(x, plan):
+    """Copies tokens to their rows: rows[plan.position[t, j]] = x[t].
+
+    x [tokens, hidden] in float32, float16 or bfloat16; returns [tokens * k,
+    hidden]. The rows of copies for no expert, behind plan.offsets[-1], are
+    zeros. Differentiable."""
+    _tensor(x, "x", 2, _FLOATS)
+    position = _check_plan(plan, x.shape[0], x)
+    _gpu(x, "pack")
+    return _Pack.apply(x, position)
+
+
+def pack_fp8(x, plan):
+    """`pack` in 8 bits: (rows [tokens * k, hidden] float8_e4m3fn, scales
+    [tokens * k, ceil(hidden / 128)] float8_e8m0fnu), quantised as
+    `quantize_fp8` does it, in the same pass over x. Rows of copies for no
+    expert are zeros, with scales of 1. It has no gradient."""
+    _tensor(x, "x", 2, _FLOATS)
+    _no_gradient("pack_fp8", x)
+    position = _check_plan(plan, x.shape[0], x)
+    _gpu(x, "pack_fp8")
+    x = _adjacent(x.detach())
+    hidden, n = x.shape[1], position.numel()
+    q, stride = _fp8_rows((n,), hidden, x.device)
+    scales = torch.empty(n, _blocks(hidden), dtype=torch.uint8,
+                         device=x.device)
+    if n and hidden:
+        _C.hip_expert_pack_fp8(
+            *_rows_args(position, hidden, x.dtype), x.data_ptr(),
+            x.stride(0), q.data_ptr(), stride, scales.data_ptr(),
+            x.get_device(), _stream(x))
+    return q, scales.view(FP8_SCALE)
+
+
+def combine(rows, plan, weights=None):
+    """Adds each token's rows up: out[t] = sum over j of weights[t, j] *
+    rows[plan.position[t, j]], in float32 and rounded once; copies for no
+    expert count nothing, and neither rows nor weights of theirs are read.
+
+    rows [tokens * k, hidden] in float32, float16 or bfloat16, weights
+    [tokens, k] float32 (all 1 if None); returns [tokens, hidden].
+    Differentiable with respect to rows and weights."""
+    _tensor(rows, "rows", 2, _FLOATS)
+    position = _check_plan(plan, None, rows)
+    _need(rows.shape[0] == position.numel(),
+          f"rows: the plan has {position.numel()}, got {rows.shape[0]}")
+    if weights is not None:
+        _tensor(weights, "weights", 2, (torch.float32,), rows)
+        _need(weights.shape == position.shape,
+              f"weights: {tuple(position.shape)} is needed, got "
+              f"{tuple(weights.shape)}")
+        weights = weights.contiguous()
+    _gpu(rows, "combine")
+    return _Combine.apply(rows, position, weights)
+
+
+# ------------------------------------------------------------ 8-bit products
+
+
+def _no_gradient(name, *tensors):
+    _need(not (torch.is_grad_enabled()
+               and any(t.requires_grad for t in tensors)),
+          f"{name} has no gradient: detach() its inputs")
+
+
+def _fp8_rows(shape, width, device):
+    """Room for rows of `width` 8-bit values that begin on borders of 128
+    bytes, so that products can load them whole."""
+    stride = _blocks(width) * FP8_BLOCK
+    q = torch.empty(*shape, stride, dtype=torch.uint8, device=device)
+    return q.view(FP8)[..., :width], stride
+
+
+def quantize_fp8(x, tile=False):
+    """8-bit values of x and their scales: x is about q * scale.
+
+    x [rows, cols] in float32, float16 or bfloat16, of any strides. A scale
+    is for 128 elements of a row: returns (q [rows, cols] float8_e4m3fn,
+    scales [rows, ceil(cols / 128)] float8_e8m0fnu). With `tile` it is for
+    128 x 128 elements, as weights have it, scales are [ceil(rows / 128),
+    ceil(cols / 128)], and x may have a leading dimension for experts. For
+    scales along the columns (a weight gradient's operands) quantise x.t().
+    Rows of q begin on borders of 128 bytes. It has no gradient."""
+    if tile and isinstance(x, torch.Tensor) and x.dim() == 3:
+        _tensor(x, "x", 3, _FLOATS)
+        _no_gradient("quantize_fp8", x)
+        _gpu(x, "quantize_fp8")
+        experts, rows, cols = x.shape
+        q, stride = _fp8_rows((experts, rows), cols, x.device)
+        scales = torch.empty(experts, _blocks(rows), _blocks(cols),
+                             dtype=torch.uint8, device=x.device)
+        for e in range(experts):
+            _quantize(x[e], True, q[e], stride, scales[e])
+        return q, scales.view(FP8_SCALE)
+    _tensor(x, "x", 2, _FLOATS)
+    _no_gradient("quantize_fp8", x)
+    _gpu(x, "quantize_fp8")
+    rows, cols = x.shape
+    q, stride = _fp8_rows((rows,), cols, x.device)
+    scales = torch.empty(_blocks(rows) if tile else rows, _blocks(cols),
+                         dtype=torch.uint8, device=x.device)
+    _quantize(x, bool(tile), q, stride, scales)
+    return q, scales.view(FP8_SCALE)
+
+
+def _quantize(x, tile, q, stride, scales):
+    x = x.detach()
+    _need(x.shape[1] <= 65535 * FP8_BLOCK,
+          f"quantize_fp8: at most {65535 * FP8_BLOCK} columns, got "
+          f"{x.shape[1]}")
+    if x.numel():
+        _C.hip_quantize_fp8(
+            x.data_ptr(), x.stride(0), x.stride(1), _FLOATS[x.dtype],
+            x.shape[0], x.shape[1], tile, q.data_ptr(), stride,
+            scales.data_ptr(), x.get_device(), _stream(x))
+
+
+def _fp8_operand(q, scale, name, dim, scale_shape, like=None):
+    _tensor(q, name, dim, (FP8,), like)
+    _tensor(scale, f"{name}_scale", dim, (FP8_SCALE,), q)
+    _need(tuple(scale.shape) == scale_shape,
+          f"{name}_scale: {scale_shape} is needed, got "
+          f"{tuple(scale.shape)}")
+    return _adjacent(q), scale.contiguous()
+
+
+def _offsets(offsets, experts, like):
+    if offsets is None:
+        return 0
+    _tensor(offsets, "offsets", 1, (torch.int32,), like)
+    _need(offsets.shape[0] == experts + 1 and offsets.is_contiguous(),
+          f"offsets: {experts + 1} adjacent numbers are needed, got "
+          f"{tuple(offsets.shape)}")
+    return offsets.data_ptr()
+
+
+def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
+    """Products of rows with weights in 8 bits: a b^T, or each expert's.
+
+    a [rows, inner] float8_e4m3fn with a scale for each 128 of a row
+    (a_scale [rows, ceil(inner / 128)] float8_e8m0fnu), b [n, inner] with one
+    for each 128 x 128 (b_scale [ceil(n / 128), ceil(inner / 128)]): returns
+    [rows, n] in `dtype` (float32, float16 or bfloat16), added up in float32
+    and rounded once. With `offsets` (int32 [experts + 1], a plan's) b and
+    b_scale have a leading dimension for experts, and rows offsets[e] to
+    offsets[e + 1] are multiplied by b[e]; rows behind the last expert's are
+    zeros. The data gradient is the same product with the weights'
+    transposed copy; `fp8_weight_grad` is the other one."""
+    _need(isinstance(a, torch.Tensor) and a.dim() == 2,
+          "a: a tensor of 2 dimensions is needed")
+    _need(isinstance(b, torch.Tensor)
+          and b.dim() == (2 if offsets is None else 3),
+          "b: [n, inner], or [experts, n, inner] with offsets")
+    _need(dtype in _FLOATS, f"fp8_matmul: cannot return {dtype}")
+    rows, inner = a.shape
+    n = b.shape[-2]
+    experts = 1 if offsets is None else b.shape[0]
+    _need(b.shape[-1] == inner,
+          f"b: an inner dimension of {inner} is needed, got {b.shape[-1]}")
+    _need(n > 0 and experts > 0, f"b: got {tuple(b.shape)}")
+    a, a_scale = _fp8_operand(a, a_scale, "a", 2, (rows, _blocks(inner)))
+    b, b_scale = _fp8_operand(
+        b, b_scale, "b", b.dim(),
+        tuple(b.shape[:-2]) + (_blocks(n), _blocks(inner)), a)
+    at = _offsets(offsets, experts, a)
+    _gpu(a, "fp8_matmul")
+    out = torch.empty(rows, n, dtype=dtype, device=a.device)
+    if rows:
+        _C.hip_fp8_matmul(
+            a.data_ptr(), a.stride(0), a_scale.data_ptr(), b.data_ptr(),
+            b.stride(-2), 0 if offsets is None else b.stride(0),
+            b_scale.data_ptr(), at, rows, n, inner, experts, out.data_ptr(),
+            _FLOATS[dtype], a.get_device(), _stream(a))
+    return out
+
+
+def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
+                    dtype=torch.float32):
+    """The weights' gradient dy x^T in 8 bits, or each expert's.
+
+    dy [m, rows] and x [n, rows] float8_e4m3fn with a scale for each 128 of
+    the rows (dy_scale [m, ceil(rows / 128)], x_scale [n, ...]), which is
+    what quantize_fp8 makes of the transposed matrices: returns [m, n] in
+    `dtype`, added up in float32 and rounded once. With `offsets` (int32
+    [experts + 1]) rows offsets[e] to offsets[e + 1] are expert e's, and the
+    result is [experts, m, n], zeros for an expert without rows. Experts may
+    begin anywhere: two of them can share a block and its scale."""
+    _need(isinstance(dy, torch.Tensor) and dy.dim() == 2
+          and isinstance(x, torch.Tensor) and x.dim() == 2,
+          "dy, x: tensors of 2 dimensions are needed")
+    _need(dtype in _FLOATS, f"fp8_weight_grad: cannot return {dtype}")
+    (m, rows), n = dy.shape, x.shape[0]
+    _need(x.shape[1] == rows, f"x: {rows} rows are needed, got {x.shape[1]}")
+    _need(m > 0 and n > 0, f"dy, x: got {tuple(dy.shape)}, "
+          f"{tuple(x.shape)}")
+    dy, dy_scale = _fp8_operand(dy, dy_scale, "dy", 2, (m, _blocks(rows)))
+    x, x_scale = _fp8_operand(x, x_scale, "x", 2, (n, _blocks(rows)), dy)
+    experts = 1
+    if offsets is not None:
+        _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1
+              and offsets.shape[0] > 1, "offsets: [experts + 1] is needed")
+        experts = offsets.shape[0] - 1
+    at = _offsets(offsets, experts, dy)
+    _gpu(dy, "fp8_weight_grad")
+    out = torch.empty((m, n) if offsets is None else (experts, m, n),
+                      dtype=dtype, device=dy.device)
+    _C.hip_fp8_weight_grad(
+        dy.data_ptr(), dy.stride(0), dy_scale.data_ptr(), x.data_ptr(),
+        x.stride(0), x_scale.data_ptr(), at, m, n, rows, experts,
+        out.data_ptr(), _FLOATS[dtype], dy.get_device(), _stream(dy))
+    return out

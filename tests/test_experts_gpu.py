@@ -1,0 +1,926 @@
+"""Expert-parallel operators and 8-bit products on the GPU, against plain
+implementations in 64 bits.
+
+Tolerances count roundings: one to a type t is off by at most
+finfo(t).eps / 2 of the value, a sum of n terms in 32 bits by n * 2^-24 of
+the sum of the terms' absolute values.
+"""
+import math
+
+import numpy as np
+import pytest
+
+import gloo_amd as ga
+
+torch = pytest.importorskip("torch")
+
+from gloo_amd import experts as ex  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("no GPU", allow_module_level=True)
+
+F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+U = 2.0 ** -24  # half a step of fp32
+DTYPES = [torch.float32, torch.float16, torch.bfloat16]
+
+
+def half_step(dtype):
+    return torch.finfo(dtype).eps / 2
+
+
+def rounded(got, ref, slack=0.0):
+    """got is ref (64 bits) rounded to its type, `slack` off before that."""
+    tiny = torch.finfo(got.dtype).smallest_normal * half_step(got.dtype) * 2
+    err = (got.double().cpu() - ref).abs()
+    most = (ref.abs() + slack) * half_step(got.dtype) + slack + tiny
+    assert torch.isfinite(err).all()
+    worst = (err - most).max() if err.numel() else torch.tensor(-1.0)
+    assert worst <= 0, f"off by {worst:.3g} more than the roundings"
+
+
+# ------------------------------------------------------------------- router
+
+
+def route_ref(x, k, score, bias, groups, topk_groups, group_score,
+              renormalize, scale):
+    """Row by row in 64 bits. Returns weights, ids."""
+    x = x.double().cpu().numpy()
+    t, e = x.shape
+    w, ids = np.zeros((t, k)), np.full((t, k), -1)
+    b = np.zeros(e) if bias is None else bias.double().cpu().numpy()
+    per = e // groups
+    for r in range(t):
+        row = np.minimum(x[r], float(torch.finfo(torch.float32).max))
+        alive = row > -np.inf  # False for NaN
+        if not alive.any():
+            continue
+        if score == "softmax":
+            p = np.where(alive, np.exp(np.where(alive, row, 0)
+                                       - row[alive].max()), 0)
+            s = p / p.sum()
+        else:
+            with np.errstate(over="ignore"):
+                s = np.where(alive, 1 / (1 + np.exp(-np.where(
+                    alive, row, 0))), 0)
+        value = np.where(alive, s + b, -np.inf)
+        rank = np.where(alive, row, -np.inf) if bias is None else value
+        if groups > 1:
+            if group_score == "max":
+                of = rank.reshape(groups, per).max(1)
+            else:
+                v = -np.sort(-value.reshape(groups, per), axis=1)[:, :2]
+                of = v[:, 0] + np.where(v[:, -1] > -np.inf, v[:, -1], 0) * (
+                    per > 1)
+            keep = np.argsort(-of, kind="stable")[:topk_groups]
+            for g in range(groups):
+                if g not in keep:
+                    rank[g * per:(g + 1) * per] = -np.inf
+        order = np.argsort(-rank, kind="stable")[:k]
+        order = [i for i in order if rank[i] > -np.inf]
+        ids[r, :len(order)] = order
+        w[r, :len(order)] = s[order]
+        if renormalize and w[r].sum() > 0:
+            w[r] /= w[r].sum()
+    return torch.from_numpy(w * scale), torch.from_numpy(ids)
+
+
+ROUTES = [
+    # tokens, experts, k, score, bias, groups, kept, group_score, renorm
+    (1, 1, 1, "softmax", False, 1, 1, "max", True),
+    (3, 8, 2, "softmax", False, 1, 1, "max", True),
+    (5, 8, 8, "softmax", True, 1, 1, "max", False),
+    (67, 60, 4, "softmax", False, 1, 1, "max", False),
+    (33, 64, 6, "softmax", True, 8, 3, "max", False),
+    (130, 256, 8, "sigmoid", True, 8, 4, "top2", True),
+    (9, 256, 8, "sigmoid", False, 8, 4, "top2", True),
+    (9, 160, 6, "softmax", False, 8, 3, "top2", False),
+    (17, 51, 5, "sigmoid", True, 3, 2, "max", False),
+    (6, 1024, 64, "sigmoid", True, 64, 32, "top2", True),
+    (6, 1000, 10, "softmax", False, 1, 1, "max", True),
+    (4, 6, 3, "sigmoid", True, 6, 3, "top2", True),
+    (40, 96, 3, "softmax", True, 4, 1, "top2", True),
+    (257, 128, 1, "sigmoid", False, 1, 1, "max", True),
+]
+
+
+def logits_of(tokens, experts, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(tokens, experts, generator=gen) * 2
+    return x.to(dtype).cuda(), gen
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", ROUTES)
+def test_route(case, dtype):
+    t, e, k, score, has_bias, groups, kept, gs, renorm = case
+    x, gen = logits_of(t, e, dtype)
+    bias = (torch.randn(e, generator=gen) * 0.3).cuda() if has_bias else None
+    w, ids = ex.route(x, k, score=score, bias=bias, groups=groups,
+                      topk_groups=kept, group_score=gs, renormalize=renorm,
+                      scale=1.5)
+    ref, rid = route_ref(x, k, score, bias, groups, kept, gs, renorm, 1.5)
+    assert ids.dtype == torch.int32 and w.dtype == torch.float32
+    assert torch.equal(ids.cpu().long(), rid)
+    # scores in 64 bits: one rounding, and 2^-44 for their own arithmetic
+    rounded(w, ref, ref.abs().max().item() * 2.0 ** -44)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("has_bias", [False, True])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_masks_and_extremes(score, has_bias, renorm):
+    inf, low = math.inf, torch.finfo(torch.float32).min
+    x, gen = logits_of(12, 16, torch.float32)
+    x = x.cpu()
+    x[0] = -inf  # nothing left
+    x[1, 1:] = -inf  # one left
+    x[2, 3:] = -inf  # fewer than k
+    x[3] = low  # the type's lowest value is a value
+    x[4, 5:] = low
+    x[5, 2] = math.nan
+    x[6] = math.nan
+    x[7, 3] = inf
+    x[8] = inf
+    x[9] = 0.25  # all the same: the lowest numbers
+    x[10, ::2] = 30.0  # where sigmoid rounds to 1 in 32 bits
+    x[10, 1::2] = 31.0
+    x[11] = -200.0
+    bias = torch.zeros(16)
+    bias[7] = -inf  # never chosen
+    bias = bias.cuda() if has_bias else None
+    x = x.cuda()
+    for groups, kept in ((1, 1), (4, 2)):
+        for gs in ("max", "top2"):
+            args = (score, bias, groups, kept, gs, renorm, 2.0)
+            w, ids = ex.route(x, 4, score=score, bias=bias, groups=groups,
+                              topk_groups=kept, group_score=gs,
+                              renormalize=renorm, scale=2.0)
+            ref, rid = route_ref(x, 4, *args)
+            # a place in row 11 where 64 bits hold differences of 1e-87
+            assert torch.equal(ids.cpu().long(), rid)
+            rounded(w, ref, 2.0 ** -44)
+
+
+def test_route_strides_and_sizes():
+    x, _ = logits_of(40, 64, torch.bfloat16)
+    wide = torch.randn(40, 200, device="cuda").bfloat16()
+    for view in (wide[:, 7:71], x[::3], x.t().contiguous().t(),
+                 x[:1].expand(5, 64), x[:0], x[:1]):
+        w, ids = ex.route(view, 4)
+        rw, rid = ex.route(view.contiguous(), 4)
+        assert torch.equal(ids, rid) and torch.equal(w, rw)
+        assert w.shape == (view.shape[0], 4)
+
+
+GRADS = [c for c in ROUTES if c[2] > 1]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("case", GRADS)
+def test_route_gradient(case, dtype):
+    t, e, k, score, has_bias, groups, kept, gs, renorm = case
+    x, gen = logits_of(t, e, dtype, seed=1)
+    bias = (torch.randn(e, generator=gen) * 0.3).cuda() if has_bias else None
+    x.requires_grad_()
+    w, ids = ex.route(x, k, score=score, bias=bias, groups=groups,
+                      topk_groups=kept, group_score=gs, renormalize=renorm,
+                      scale=1.5)
+    g = torch.randn(t, k, generator=gen).cuda()
+    dx, = torch.autograd.grad(w, x, g)
+    assert dx.dtype == dtype and not ids.requires_grad
+    y = x.detach().double().cpu().requires_grad_()
+    s = torch.softmax(y, 1) if score == "softmax" else torch.sigmoid(y)
+    v = s.gather(1, ids.cpu().long())
+    v = v / v.sum(1, keepdim=True) if renorm else v
+    ref, = torch.autograd.grad(v * 1.5, y, g.double().cpu())
+    # 64 bits until the last rounding; differences of terms of this size
+    slack = g.abs().max().item() * 1.5 * k * 2.0 ** -40
+    rounded(dx, ref, slack + U * ref.abs().max().item())
+
+
+def test_route_gradient_of_masked_rows():
+    x, gen = logits_of(6, 16, torch.float32)
+    x[0] = -math.inf
+    x[1, 2:] = -math.inf
+    x[2, 1:] = -math.inf
+    x[3, 4] = math.nan
+    x[4, 4] = math.inf
+    for score in ("softmax", "sigmoid"):
+        for renorm in (False, True):
+            y = x.clone().requires_grad_()
+            w, ids = ex.route(y, 4, score=score, renormalize=renorm)
+            w.sum().backward()  # an expanded gradient
+            got = y.grad
+            assert torch.isfinite(got).all()
+            assert (got[0] == 0).all() and (got[1, 2:] == 0).all()
+            assert got[3, 4] == 0
+            if renorm:  # the weights' sum is 1 whatever the logits are
+                assert got.abs().max() <= 4 * 2.0 ** -50
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renorm", [False, True])
+def test_route_gradient_by_differences(score, renorm):
+    """The loss along a direction d (|d| <= 1): central differences are off
+    by h^2 / 6 of its third derivative (below 8 for each weight) and by the
+    weights' rounding over h."""
+    gen = torch.Generator().manual_seed(3)
+    t, e, k, h = 8, 32, 4, 2.0 ** -7
+    # logits at least 0.1 apart: the steps do not change who is chosen
+    x = torch.stack([torch.randperm(e, generator=gen) for _ in range(t)])
+    x = (x.float() * 0.1 - 2).cuda().requires_grad_()
+    d = (torch.rand(t, e, generator=gen) * 2 - 1).cuda()
+    g = torch.randn(t, k, generator=gen).cuda()
+    w, ids = ex.route(x, k, score=score, renormalize=renorm)
+    dx, = torch.autograd.grad(w, x, g)
+    loss = []
+    for sign in (1, -1):
+        y, at = ex.route(x.detach() + sign * h * d, k, score=score,
+                         renormalize=renorm)
+        assert torch.equal(at, ids)
+        loss.append((y.double() * g).sum().item())
+    slope = (loss[0] - loss[1]) / (2 * h)
+    size = g.abs().sum().item()
+    # x + h d is rounded too: 2^-24 of |x| <= 2
+    most = size * (2 * U / h + 2 * U / h + h * h * 8 / 6)
+    assert abs(slope - (dx.double() * d).sum().item()) <= most
+
+
+# ----------------------------------------------------- plan, pack, combine
+
+
+def ids_of(t, k, e, gen, dropped=0.0):
+    ids = torch.stack([torch.randperm(max(e, k), generator=gen)[:k] % e
+                       for _ in range(t)]) if t else torch.zeros(0, k)
+    ids = ids.reshape(t, k).to(torch.int32)
+    if dropped:
+        ids[torch.rand(t, k, generator=gen) < dropped] = -1
+    return ids
+
+
+def plan_ref(ids, e):
+    flat = ids.reshape(-1).numpy().astype(np.int64)
+    key = np.where((flat < 0) | (flat >= e), e, flat)
+    order = np.argsort(key, kind="stable")
+    place = np.empty_like(order)
+    place[order] = np.arange(len(order))
+    counts = np.bincount(key, minlength=e + 1)[:e]
+    place = np.where(key == e, ~place, place)
+    return (torch.from_numpy(place).view(ids.shape), torch.from_numpy(counts),
+            torch.from_numpy(np.concatenate([[0], np.cumsum(counts)])))
+
+
+def same_plan(p, ids, e):
+    place, counts, offsets = plan_ref(ids, e)
+    assert torch.equal(p.position.cpu().long(), place)
+    assert torch.equal(p.counts.cpu().long(), counts)
+    assert torch.equal(p.offsets.cpu().long(), offsets)
+
+
+@pytest.mark.parametrize("t,k,e", [
+    (0, 2, 8), (1, 1, 1), (1, 8, 256), (7, 3, 5), (64, 1, 64), (65, 2, 63),
+    (511, 4, 64), (512, 4, 3), (513, 4, 1024), (3000, 8, 256), (40000, 1, 7),
+    (70001, 8, 300),
+])
+@pytest.mark.parametrize("dropped", [0.0, 0.3, 1.0])
+def test_plan(t, k, e, dropped):
+    gen = torch.Generator().manual_seed(t + e)
+    if t > 10000:
+        ids = torch.randint(0, e, (t, k), generator=gen, dtype=torch.int32)
+        ids[torch.rand(t, k, generator=gen) < dropped] = -1
+    else:
+        ids = ids_of(t, k, e, gen, dropped)
+    same_plan(ex.plan(ids.cuda(), e), ids, e)
+
+
+def test_plan_of_odd_ids():
+    """Numbers that are no expert, one expert for all, the same one twice
+    for a token, and ids that are not adjacent in memory."""
+    ids = torch.tensor([[5, 5], [-7, 8], [2 ** 31 - 1, 0], [-2 ** 31, 7]],
+                       dtype=torch.int32)
+    same_plan(ex.plan(ids.cuda(), 8), ids, 8)
+    one = torch.full((5000, 2), 3, dtype=torch.int32)
+    same_plan(ex.plan(one.cuda(), 4), one, 4)
+    gen = torch.Generator().manual_seed(5)
+    wide = torch.randint(-1, 16, (100, 6), generator=gen, dtype=torch.int32)
+    same_plan(ex.plan(wide.cuda()[:, ::2], 16), wide[:, ::2], 16)
+
+
+ROWS = [(1, 1, 1, 8), (1, 8, 16, 4096), (5, 3, 4, 1), (33, 2, 8, 100),
+        (64, 8, 64, 512), (77, 9, 12, 1000), (130, 4, 8, 2056),
+        (3, 17, 20, 8200), (300, 6, 60, 136)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,k,e,h", ROWS)
+@pytest.mark.parametrize("dropped", [0.0, 0.4])
+def test_pack_and_combine(t, k, e, h, dtype, dropped):
+    gen = torch.Generator().manual_seed(h)
+    ids = ids_of(t, k, e, gen, dropped)
+    p = ex.plan(ids.cuda(), e)
+    place = plan_ref(ids, e)[0]
+    real = place >= 0
+    x = torch.randn(t, h, generator=gen).to(dtype)
+    xg = x.cuda().requires_grad_()
+    rows = ex.pack(xg, p)
+    expect = torch.zeros(t * k, h, dtype=dtype)
+    expect[place[real]] = x.repeat_interleave(k, 0).view(t, k, h)[real]
+    assert torch.equal(rows.detach().cpu(), expect)
+    # gradient: a sum of at most k terms in 32 bits
+    g = torch.randn(t * k, h, generator=gen).to(dtype)
+    dx, = torch.autograd.grad(rows, xg, g.cuda())
+    each = g.double()[torch.where(real, place, ~place)] * real[..., None]
+    rounded(dx, each.sum(1), (k * U * each.abs().sum(1)).max().item())
+
+    w = torch.rand(t, k, generator=gen) - 0.3
+    yg, wg = g.cuda().requires_grad_(), w.cuda().requires_grad_()
+    out = ex.combine(yg, p, wg)
+    terms = each * w.double()[..., None]
+    ref = terms.sum(1)
+    err = (out.double().cpu() - ref).abs()
+    most = (half_step(dtype) * ref.abs()
+            + (1 + half_step(dtype)) * k * U * terms.abs().sum(1) + 1e-30)
+    if dtype == torch.float16:
+        most = most + 2.0 ** -25  # below its normal numbers
+    assert (err <= most).all()
+    og = torch.randn(t, h, generator=gen).to(dtype)
+    drows, dw = torch.autograd.grad(out, (yg, wg), og.cuda())
+    refd = torch.zeros(t * k, h, dtype=torch.float64)
+    refd[place[real]] = (og.double()[:, None] * w.double()[..., None])[real]
+    rounded(drows, refd, U * refd.abs().max().item())
+    prod = each * og.double()[:, None]
+    assert ((dw.double().cpu() - prod.sum(2)).abs()
+            <= (h + 1) * U * prod.abs().sum(2)).all()
+    assert (dw.cpu()[~real] == 0).all()
+    # without weights: sums
+    plain = ex.combine(yg, p)
+    rounded(plain.detach(), each.sum(1),
+            (k * U * each.abs().sum(1)).max().item())
+    dplain, = torch.autograd.grad(plain, yg, og.cuda())
+    refp = torch.zeros(t * k, h, dtype=dtype)
+    refp[place[real]] = og.repeat_interleave(k, 0).view(t, k, h)[real]
+    assert torch.equal(dplain.cpu(), refp)
+
+
+def test_combine_by_differences():
+    """out is linear in rows and in weights: a step of h changes the loss
+    by h times the gradient, up to the roundings of out."""
+    gen = torch.Generator().manual_seed(9)
+    t, k, e, h = 6, 3, 5, 40
+    p = ex.plan(ids_of(t, k, e, gen).cuda(), e)
+    rows = torch.randn(t * k, h, generator=gen).cuda().requires_grad_()
+    w = torch.rand(t, k, generator=gen).cuda().requires_grad_()
+    g = torch.randn(t, h, generator=gen).cuda()
+    dr, dw = torch.autograd.grad(ex.combine(rows, p, w), (rows, w), g)
+    r0, w0 = rows.detach(), w.detach()
+    r1 = torch.randn(t * k, h, generator=gen).cuda()
+    w1 = torch.randn(t, k, generator=gen).cuda()
+    for a, b, slope in (
+            ((r0 + r1, w0), (r0 - r1, w0), (dr.double() * r1).sum()),
+            ((r0, w0 + w1), (r0, w0 - w1), (dw.double() * w1).sum())):
+        hi, lo = (ex.combine(x, p, y).double() for x, y in (a, b))
+        size = (g.abs() * (hi.abs() + lo.abs() + 12 * k)).sum().item()
+        got = ((hi - lo) * g).sum().item() / 2
+        assert abs(got - slope.item()) <= 8 * k * U * size
+
+
+def test_rows_of_odd_strides():
+    gen = torch.Generator().manual_seed(4)
+    ids = ids_of(20, 4, 8, gen)
+    p = ex.plan(ids.cuda(), 8)
+    wide = torch.randn(20, 300, generator=gen).cuda().bfloat16()
+    cases = [wide[:, 3:131], wide[:, ::2][:, :128], wide[:, 8:136],
+             wide[:1, :128].expand(20, 128),
+             wide[:, :128].t().contiguous().t()]
+    for x in cases:
+        assert torch.equal(ex.pack(x, p), ex.pack(x.contiguous(), p))
+        q, s = ex.pack_fp8(x, p)
+        rq, rs = ex.pack_fp8(x.contiguous(), p)
+        assert torch.equal(q.float(), rq.float())
+        assert torch.equal(s.float(), rs.float())
+    rows = torch.randn(80, 300, generator=gen).cuda().half()
+    w = torch.rand(4, 20, generator=gen).cuda().t()
+    for y in (rows[:, 5:133], rows[:, 8:136], rows[:1, :128].expand(80, 128)):
+        assert torch.equal(ex.combine(y, p, w),
+                           ex.combine(y.contiguous(), p, w.contiguous()))
+
+
+def test_combine_skips_what_is_masked():
+    """Rows of copies for no expert may hold anything."""
+    ids = torch.tensor([[0, -1], [-1, -1], [1, 0]], dtype=torch.int32).cuda()
+    p = ex.plan(ids, 2)
+    rows = torch.ones(6, 8, device="cuda")
+    rows[3:] = math.nan
+    w = torch.full((3, 2), math.nan, device="cuda")
+    w[0, 0], w[2] = 2.0, 0.5
+    rows.requires_grad_(), w.requires_grad_()
+    out = ex.combine(rows, p, w)
+    assert torch.equal(out[:, 0].cpu(), torch.tensor([2.0, 0.0, 1.0]))
+    dr, dw = torch.autograd.grad(out, (rows, w), torch.ones_like(out))
+    assert torch.isfinite(dr).all() and torch.isfinite(dw).all()
+    assert (dr[3:] == 0).all() and (dw[1] == 0).all() and dw[0, 1] == 0
+
+
+def test_large_offsets():
+    """Rows past 2^31 elements and 2^32 bytes."""
+    t, k, h = 70000, 8, 4096
+    ids = torch.arange(k, device="cuda", dtype=torch.int32).repeat(t, 1)
+    p = ex.plan(ids, k)
+    x = torch.zeros(t, h, dtype=torch.bfloat16, device="cuda")
+    x[:] = torch.arange(t, device="cuda")[:, None] % 251
+    rows = ex.pack(x, p)
+    assert rows.numel() > 2 ** 31
+    at = torch.tensor([0, 1, t - 1, t, 5 * t + 77, 8 * t - 1])
+    assert torch.equal(rows[at.cuda()][:, ::511].float().cpu(),
+                       (at % t % 251).float()[:, None].expand(6, 9))
+    out = ex.combine(rows, p)  # 8 equal rows each: up to 2000, exact in 32
+    ref = (x[:, 0].float() * 8).bfloat16()
+    assert torch.equal(out[:, 0], ref) and torch.equal(out[:, -1], ref)
+
+
+# ------------------------------------------------------------ 8-bit products
+
+
+GRID = torch.arange(256, dtype=torch.uint8).view(F8).double()
+GRID = torch.sort(GRID[torch.isfinite(GRID)].unique()).values.numpy()
+
+
+def to_e4m3(v):
+    """Nearest of the 8-bit values, ties to the one with an even last bit
+    (every other one from zero on)."""
+    v = np.asarray(v, dtype=np.float64)
+    pos = GRID[GRID >= 0]
+    a = np.abs(v)
+    hi = np.clip(np.searchsorted(pos, a), 0, len(pos) - 1)
+    lo = np.clip(hi - 1, 0, None)
+    up, down = pos[hi] - a, a - pos[lo]
+    pick = np.where((up < down) | ((up == down) & (hi % 2 == 0)), hi, lo)
+    return np.sign(v) * pos[pick]
+
+
+def quant_ref(x, br=1):
+    """(values, scales) in 64 bits, blocks of br x 128."""
+    x = x.double().cpu().numpy()
+    r, c = x.shape
+    q = np.zeros_like(x)
+    s = np.ones((-(-r // br), -(-c // 128)))
+    for i in range(s.shape[0]):
+        for j in range(s.shape[1]):
+            part = np.s_[i * br:(i + 1) * br, j * 128:(j + 1) * 128]
+            top = np.abs(x[part]).max()
+            if top > 0:
+                e = -127
+                while top / 2.0 ** e > 448:
+                    e += 1
+                s[i, j] = 2.0 ** e
+            q[part] = to_e4m3(x[part] / s[i, j])
+    return torch.from_numpy(q), torch.from_numpy(s)
+
+
+def same_quant(got, ref):
+    (q, s), (rq, rs) = got, ref
+    assert q.dtype == F8 and s.dtype == E8
+    assert torch.equal(s.double().cpu(), rs)
+    assert torch.equal(q.double().cpu(), rq)
+
+
+def some(r, c, dtype, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(r, c, generator=gen)
+    x *= torch.exp2(torch.randint(-9, 6, (r, 1), generator=gen).float())
+    if r > 2 and c > 5:
+        x[1] = 0
+        x[2, :5] = torch.tensor([448.0, 448.5, 449.0, 464.0, 480.0])
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r,c", [(1, 1), (1, 128), (3, 16), (5, 100),
+                                 (64, 256), (65, 257), (130, 1000),
+                                 (200, 384)])
+def test_quantize(r, c, dtype):
+    x = some(r, c, dtype)
+    g = x.cuda()
+    ref = quant_ref(x)
+    got = ex.quantize_fp8(g)
+    same_quant(got, ref)
+    assert got[0].stride(0) % 128 == 0
+    same_quant(ex.quantize_fp8(g.t().contiguous().t()), ref)  # by columns
+    wide = torch.zeros(r, c + 9, dtype=dtype, device="cuda")
+    wide[:, 5:5 + c] = g
+    same_quant(ex.quantize_fp8(wide[:, 5:5 + c]), ref)
+    same_quant(ex.quantize_fp8(g, tile=True), quant_ref(x, 128))
+    same_quant(ex.quantize_fp8(g.t().contiguous().t(), tile=True),
+               quant_ref(x, 128))
+
+
+def test_quantize_extremes():
+    x = torch.zeros(9, 256)
+    x[0, 0], x[0, 1] = 2.0 ** -140, 2.0 ** -149  # below the normal numbers
+    x[1, :3] = torch.tensor([3e38, -3.4e38, 1e30])
+    x[2, 7] = 2.0 ** -126
+    x[3, 0] = 448 * 2.0 ** -3
+    x[3, 200] = -(448 * 2.0 ** -3) * (1 + 2.0 ** -20)
+    x[4] = 1e-30
+    x[5, :128] = 1e-38
+    same_quant(ex.quantize_fp8(x.cuda()), quant_ref(x))
+    x[6, 5], x[7, 130], x[8, 0] = math.inf, math.nan, -math.inf
+    q, s = ex.quantize_fp8(x.cuda())
+    bad = torch.zeros(9, 2, dtype=torch.bool)
+    bad[6, 0] = bad[7, 1] = bad[8, 0] = True
+    assert torch.equal(torch.isnan(s.float().cpu()), bad)
+    assert torch.isnan(q.float().cpu()[6, 5])
+
+
+def test_quantize_of_experts():
+    w = torch.randn(3, 200, 300).cuda()
+    q, s = ex.quantize_fp8(w, tile=True)
+    assert q.shape == w.shape and s.shape == (3, 2, 3)
+    for e in range(3):
+        same_quant((q[e], s[e]), quant_ref(w[e].cpu(), 128))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,k,e,h", ROWS)
+def test_pack_fp8(t, k, e, h, dtype):
+    gen = torch.Generator().manual_seed(h)
+    ids = ids_of(t, k, e, gen, 0.2)
+    x = some(t, h, dtype, h)
+    p = ex.plan(ids.cuda(), e)
+    place = plan_ref(ids, e)[0]
+    real = place >= 0
+    rq, rs = quant_ref(x)
+    q = torch.zeros(t * k, h, dtype=torch.float64)
+    s = torch.ones(t * k, rs.shape[1], dtype=torch.float64)
+    q[place[real]] = rq.repeat_interleave(k, 0).view(t, k, -1)[real]
+    s[place[real]] = rs.repeat_interleave(k, 0).view(t, k, -1)[real]
+    same_quant(ex.pack_fp8(x.cuda(), p), (q, s))
+
+
+def operand(shape, scale_shape, gen):
+    """8-bit values and scales of 2^-6 to 2^6."""
+    q = (torch.randn(shape, generator=gen) * 60).clamp(-448, 448).to(F8)
+    s = torch.exp2(torch.randint(-6, 7, scale_shape,
+                                 generator=gen).float()).to(E8)
+    return q, s
+
+
+def wide_scale(s, n, dim):
+    return s.double().repeat_interleave(128, dim).narrow(dim, 0, n)
+
+
+def off_by(dtype, inner):
+    """How far sums of `inner` products may be off before the last rounding,
+    over the sum of the products' absolute values. In fp32: each addition is
+    off by a step at most (the matrix units may cut instead of rounding).
+    For 16-bit results the 8-bit matrix instruction adds products in groups
+    of eight and cuts each below 2^-13 of the group's largest: seven are cut
+    by up to 2^-13 of it, 7 * 2^-13 < 2^-10 of the group's absolute values."""
+    return 2 * U * max(1, inner) + (0 if dtype == torch.float32
+                                    else 2.0 ** -10)
+
+
+def close(got, a, b):
+    """got is a b^T, rounded once."""
+    ref, size = a @ b.t(), a.abs() @ b.abs().t()
+    err = (got.double().cpu() - ref).abs()
+    most = (half_step(got.dtype) * ref.abs() + (1 + half_step(got.dtype))
+            * off_by(got.dtype, a.shape[1]) * size)
+    assert (err <= most).all(), (err - most).max()
+
+
+def nb(n):
+    return -(-n // 128)
+
+
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1, 1), (1, 16, 16), (1, 256, 512), (2, 100, 130), (7, 128, 128),
+    (16, 4, 2064), (17, 33, 100), (31, 260, 384), (33, 512, 1040),
+    (64, 128, 256), (65, 130, 144), (128, 257, 640), (129, 128, 1000),
+    (300, 516, 96), (257, 300, 4096), (0, 16, 128), (5, 16, 0),
+])
+def test_matmul(m, n, k, out):
+    gen = torch.Generator().manual_seed(m * n + k)
+    a, sa = operand((m, k), (m, nb(k)), gen)
+    b, sb = operand((n, k), (nb(n), nb(k)), gen)
+    if out == torch.float16:  # keep what is returned inside its range
+        sa = (sa.float() * 2.0 ** -13).to(E8)
+    got = ex.fp8_matmul(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), dtype=out)
+    assert got.shape == (m, n) and got.dtype == out
+    da = a.double() * wide_scale(sa, k, 1)
+    db = b.double() * wide_scale(wide_scale(sb, n, 0).float(), k, 1)
+    if out == torch.float16:
+        ref = da @ db.t()
+        keep = ref.abs() < 60000  # and above its normal numbers' least
+        got = got.double().cpu()
+        size = da.abs() @ db.abs().t()
+        most = (half_step(out) * (ref.abs() + 2.0 ** -14)
+                + 2 * off_by(out, k) * size)
+        assert ((got - ref).abs()[keep] <= most[keep]).all()
+    else:
+        close(got, da, db)
+
+
+def test_matmul_of_whole_numbers():
+    """Small whole numbers: every sum is exact, so is the result."""
+    gen = torch.Generator().manual_seed(0)
+    for m, n, k in ((1, 64, 256), (40, 300, 384), (512, 512, 1024),
+                    (300, 1000, 528)):
+        a = torch.randint(-3, 4, (m, k), generator=gen)
+        b = torch.randint(-3, 4, (n, k), generator=gen)
+        one = torch.ones
+        got = ex.fp8_matmul(
+            a.float().to(F8).cuda(), one(m, nb(k)).to(E8).cuda(),
+            b.float().to(F8).cuda(), one(nb(n), nb(k)).to(E8).cuda(),
+            dtype=torch.float32)
+        assert torch.equal(got.cpu().double(), (a.double() @ b.double().t()))
+        got = ex.fp8_weight_grad(
+            a.float().to(F8).cuda(), one(m, nb(k)).to(E8).cuda(),
+            b.float().to(F8).cuda(), one(n, nb(k)).to(E8).cuda())
+        assert torch.equal(got.cpu().double(), (a.double() @ b.double().t()))
+
+
+GROUPS = [
+    [0, 5], [0, 0, 3], [0, 1, 1, 4, 4], [2, 7, 9], [0, 128, 256, 300],
+    [0, 3, 3, 130, 400, 401], [0] * 70 + [9], [0, 640, 641, 700],
+    list(range(0, 80)), [0, 0, 0],
+]
+
+
+@pytest.mark.parametrize("at", GROUPS)
+@pytest.mark.parametrize("n,k", [(16, 128), (130, 200), (256, 512)])
+def test_matmul_grouped(at, n, k):
+    gen = torch.Generator().manual_seed(len(at) + n)
+    e, m = len(at) - 1, at[-1] + 6  # rows behind the last expert
+    a, sa = operand((m, k), (m, nb(k)), gen)
+    b, sb = operand((e, n, k), (e, nb(n), nb(k)), gen)
+    off = torch.tensor(at, dtype=torch.int32).cuda()
+    got = ex.fp8_matmul(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(),
+                        offsets=off, dtype=torch.float32)
+    da = a.double() * wide_scale(sa, k, 1)
+    for i in range(e):
+        db = b[i].double() * wide_scale(
+            wide_scale(sb[i], n, 0).float(), k, 1)
+        close(got[at[i]:at[i + 1]], da[at[i]:at[i + 1]], db)
+    assert (got[at[-1]:] == 0).all()
+
+
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("at", GROUPS + [None])
+@pytest.mark.parametrize("m,n", [(16, 12), (130, 70), (256, 128)])
+def test_weight_grad(at, m, n, out):
+    gen = torch.Generator().manual_seed(m)
+    rows = 150 if at is None else at[-1] + 6
+    dy, sy = operand((m, rows), (m, nb(rows)), gen)
+    x, sx = operand((n, rows), (n, nb(rows)), gen)
+    if out == torch.float16:
+        sy = (sy.float() * 2.0 ** -13).to(E8)
+    off = None if at is None else torch.tensor(at, dtype=torch.int32).cuda()
+    got = ex.fp8_weight_grad(dy.cuda(), sy.cuda(), x.cuda(), sx.cuda(),
+                             offsets=off, dtype=out)
+    ddy = dy.double() * wide_scale(sy, rows, 1)
+    dx = x.double() * wide_scale(sx, rows, 1)
+    parts = [(0, rows)] if at is None else list(zip(at, at[1:]))
+    assert got.shape == ((m, n) if at is None else (len(parts), m, n))
+    for (i, j), one in zip(parts, [got] if at is None else got):
+        if out == torch.float16:
+            ref, size = ddy[:, i:j] @ dx[:, i:j].t(), \
+                ddy[:, i:j].abs() @ dx[:, i:j].abs().t()
+            keep = ref.abs() < 60000
+            most = (half_step(out) * (ref.abs() + 2.0 ** -14)
+                    + 2 * off_by(out, j - i) * size)
+            err = (one.double().cpu() - ref).abs()
+            assert (err[keep] <= most[keep]).all()
+        else:
+            close(one, ddy[:, i:j], dx[:, i:j])
+
+
+def test_products_of_odd_strides():
+    gen = torch.Generator().manual_seed(2)
+    a, sa = operand((20, 300), (20, 2), gen)
+    b, sb = operand((3, 70, 300), (3, 1, 2), gen)
+    off = torch.tensor([0, 4, 4, 20], dtype=torch.int32).cuda()
+    a, b, sa, sb = a.cuda(), b.cuda(), sa.cuda(), sb.cuda()
+    for i in (0, 1, 16):  # on and off a border of 16 bytes
+        pa = a.view(torch.uint8)[:, i:i + 200].view(F8)
+        pb = b.view(torch.uint8)[:, :, i:i + 200].view(F8)
+        got = ex.fp8_matmul(pa, sa, pb, sb, offsets=off)
+        ref = ex.fp8_matmul(pa.contiguous(), sa, pb.contiguous(), sb,
+                            offsets=off)
+        da = pa.double().cpu() * wide_scale(sa.cpu(), 200, 1)
+        db = pb[2].double().cpu() * wide_scale(
+            wide_scale(sb[2].cpu(), 70, 0).float(), 200, 1)
+        close(got[4:], da[4:], db)
+        close(ref[4:], da[4:], db)
+    # scales that are not adjacent, and a transposed operand
+    got = ex.fp8_matmul(a[:, :200].t().contiguous().t(), sa, b[0][:, :200],
+                        sb[0].t().contiguous().t())
+    da = a[:, :200].double().cpu() * wide_scale(sa.cpu(), 200, 1)
+    db = b[0][:, :200].double().cpu() * wide_scale(
+        wide_scale(sb[0].cpu(), 70, 0).float(), 200, 1)
+    close(got, da, db)
+
+
+def test_products_keep_nan_in_its_row():
+    gen = torch.Generator().manual_seed(2)
+    a, sa = operand((40, 200), (40, 2), gen)
+    b, sb = operand((70, 200), (1, 2), gen)
+    sa = sa.view(torch.uint8)
+    sa[3, 1] = 255  # a block that held an infinity
+    a = a.view(torch.uint8)
+    a[9, 7] = 0x7f  # NaN
+    got = ex.fp8_matmul(a.view(F8).cuda(), sa.view(E8).cuda(), b.cuda(),
+                        sb.cuda()).float().cpu()
+    bad = torch.isnan(got).all(1)
+    assert bad[3] and bad[9] and torch.isfinite(got).all(1).sum() == 38
+    # an expert's neighbours may hold NaN in the block that they share
+    dy, sy = operand((16, 40), (16, 1), gen)
+    x, sx = operand((8, 40), (8, 1), gen)
+    for t in (dy, x):
+        t.view(torch.uint8)[:, 10:20] = 0x7f
+    off = torch.tensor([0, 10, 20, 40], dtype=torch.int32).cuda()
+    got = ex.fp8_weight_grad(dy.cuda(), sy.cuda(), x.cuda(), sx.cuda(),
+                             offsets=off)
+    assert torch.isfinite(got[0]).all() and torch.isfinite(got[2]).all()
+    assert torch.isnan(got[1]).all()
+
+
+def test_offsets_that_are_wrong_stay_inside():
+    """Offsets are read on the device: wrong ones give wrong results, and
+    touch nothing outside the tensors."""
+    gen = torch.Generator().manual_seed(2)
+    a, sa = operand((20, 128), (20, 1), gen)
+    b, sb = operand((3, 70, 128), (3, 1, 1), gen)
+    guard = torch.full((3, 20, 70), 7.0, device="cuda")
+    for at in ([-5, 3, 2 ** 31 - 1, 2 ** 30], [9, 4, 2, 0],
+               [-2 ** 31, -1, -1, 99]):
+        off = torch.tensor(at, dtype=torch.int32).cuda()
+        ex.fp8_matmul(a.cuda(), sa.cuda(), b.cuda(), sb.cuda(), offsets=off)
+        dy, sy = operand((16, 20), (16, 1), gen)
+        ex.fp8_weight_grad(dy.cuda(), sy.cuda(), dy.cuda(), sy.cuda(),
+                           offsets=off)
+    torch.cuda.synchronize()
+    assert (guard == 7).all()
+
+
+def test_weights_past_32_bits():
+    """An expert's weights that begin past 2^32 bytes."""
+    e, n, k = 70, 8192, 8192
+    b = torch.zeros(e, n, k, dtype=torch.uint8, device="cuda").view(F8)
+    sb = torch.full((e, n // 128, k // 128), 127, dtype=torch.uint8,
+                    device="cuda").view(E8)
+    b[e - 1] = torch.ones(n, k, device="cuda").to(F8)
+    for rows in (3, 300):
+        a = torch.ones(rows, k, device="cuda").to(F8)
+        sa = torch.ones(rows, k // 128, device="cuda").to(E8)
+        at = [0] * e + [rows]
+        got = ex.fp8_matmul(
+            a, sa, b, sb, dtype=torch.float32,
+            offsets=torch.tensor(at, dtype=torch.int32).cuda())
+        assert (got == k).all()
+
+
+# ------------------------------------------------------------------ together
+
+
+def layer(x, router, w1, w2, bias):
+    """A layer of experts in bf16 rows, its products in plain torch."""
+    logits = x.float() @ router
+    weights, ids = ex.route(logits, 4, score="sigmoid", bias=bias, groups=4,
+                            topk_groups=2, group_score="top2", scale=2.0)
+    p = ex.plan(ids, w1.shape[0])
+    rows = ex.pack(x, p)
+    at = p.offsets.tolist()
+    parts = [torch.relu(rows[i:j] @ w1[e]) @ w2[e] for e, (i, j) in
+             enumerate(zip(at, at[1:]))]
+    return ex.combine(torch.cat(parts), p, weights)
+
+
+def test_layer_and_its_gradients():
+    """Against the same layer computed token by token in 64 bits."""
+    gen = torch.Generator().manual_seed(11)
+    t, h, f, e = 37, 24, 32, 16
+    x, router = torch.randn(t, h, generator=gen), \
+        torch.randn(h, e, generator=gen)
+    w1, w2 = (torch.randn(s, generator=gen) * 0.2
+              for s in ((e, h, f), (e, f, h)))
+    bias = torch.randn(e, generator=gen) * 0.1
+    leaves = [v.cuda().requires_grad_() for v in (x, router, w1, w2)]
+    out = layer(*leaves, bias.cuda())
+    g = torch.randn(t, h, generator=gen)
+    got = torch.autograd.grad(out, leaves, g.cuda())
+    ref = [v.double().requires_grad_() for v in (x, router, w1, w2)]
+    logits = ref[0] @ ref[1]
+    _, ids = route_ref(logits.detach(), 4, "sigmoid", bias, 4, 2, "top2",
+                       True, 2.0)
+    s = torch.sigmoid(logits).gather(1, ids)
+    s = 2.0 * s / s.sum(1, keepdim=True)
+    rows = []
+    for i in range(t):
+        rows.append(sum(s[i, j] * (torch.relu(
+            ref[0][i] @ ref[2][ids[i, j]]) @ ref[3][ids[i, j]])
+            for j in range(4)))
+    y = torch.stack(rows)
+    want = torch.autograd.grad(y, ref, g.double())
+    # fp32 sums of at most t * k terms, three products deep
+    for a, b in [(out, y)] + list(zip(got, want)):
+        assert ((a.double().cpu() - b.detach()).norm()
+                <= 4 * t * 4 * U * b.detach().norm() * 4)
+
+
+def serve(x, bias, router, w, ws):
+    """A decoding step's way through a layer in 8 bits: one product."""
+    weights, ids = ex.route(x.float() @ router, 4, score="sigmoid",
+                            bias=bias)
+    p = ex.plan(ids, w.shape[0])
+    q, s = ex.pack_fp8(x, p)
+    y = ex.fp8_matmul(q, s, w, ws, offsets=p.offsets)
+    return ex.combine(y, p, weights), ids
+
+
+def test_serving_step_captured_and_on_another_stream():
+    """One graph, replayed on changing inputs between the program's own
+    calls; the same calls on a stream of their own."""
+    gen = torch.Generator().manual_seed(12)
+    t, h, e = 9, 256, 16
+    router = torch.randn(h, e, generator=gen).cuda()
+    bias = (torch.randn(e, generator=gen) * 0.1).cuda()
+    w, ws = ex.quantize_fp8(torch.randn(e, h, h, generator=gen).cuda(),
+                            tile=True)
+    x = torch.randn(t, h, generator=gen).cuda().bfloat16()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            serve(x, bias, router, w, ws)
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out, ids = serve(x, bias, router, w, ws)
+    for i in range(4):
+        new = torch.randn(t, h, generator=gen).bfloat16()
+        x.copy_(new)
+        ref, rid = serve(x, bias, router, w, ws)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ref) and torch.equal(ids, rid)
+        with torch.cuda.stream(side):
+            there, _ = serve(x, bias, router, w, ws)
+        side.synchronize()
+        assert torch.equal(there, ref)
+
+
+def test_training_step_captured():
+    """Forward and backward of the row operators in one graph. No eager
+    graph of the same leaves is alive while it is captured."""
+    gen = torch.Generator().manual_seed(13)
+    t, h, e, k = 70, 96, 8, 2
+    x = torch.randn(t, h, generator=gen).cuda().requires_grad_()
+    z = torch.randn(t, e, generator=gen).cuda().requires_grad_()
+    g = torch.randn(t, h, generator=gen).cuda()
+
+    def step():
+        weights, ids = ex.route(z, k, renormalize=False)
+        p = ex.plan(ids, e)
+        y = ex.combine(ex.pack(x, p) * 2, p, weights)
+        return (y.detach(),) + torch.autograd.grad(y, (x, z), g)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for _ in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(t, h, generator=gen))
+            z.copy_(torch.randn(t, e, generator=gen))
+        ref = step()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(got, ref):
+            assert torch.equal(a, b)
+
+
+def test_same_results_every_time():
+    gen = torch.Generator().manual_seed(14)
+    t, k, e, h = 3000, 8, 64, 256
+    ids = ids_of(t, k, e, gen, 0.1).cuda()
+    rows = torch.randn(t * k, h, generator=gen).cuda().requires_grad_()
+    w = torch.rand(t, k, generator=gen).cuda().requires_grad_()
+    first = None
+    for _ in range(3):
+        p = ex.plan(ids, e)
+        out = ex.combine(rows, p, w)
+        got = (p.position, out.detach()) + torch.autograd.grad(
+            out, (rows, w), torch.ones_like(out))
+        first = first or got
+        assert all(torch.equal(a, b) for a, b in zip(first, got))
