@@ -243,6 +243,17 @@ struct RowTile {
   int64_t end;
 };
 
+// The same value in every lane, told to the compiler: what follows from it
+// is held once a wave.
+__device__ inline int uniform(int v) {
+  return __builtin_amdgcn_readfirstlane(v);
+}
+__device__ inline int64_t uniform(int64_t v) {
+  const uint32_t lo = uniform(static_cast<int>(v));
+  const uint32_t hi = uniform(static_cast<int>(v >> 32));
+  return static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo);
+}
+
 __device__ inline int64_t clampOffset(
     const int32_t* offsets,
     int e,
@@ -251,49 +262,115 @@ __device__ inline int64_t clampOffset(
   return v < 0 ? 0 : (v > rows ? rows : v);
 }
 
-// The tile-th tile of kBM rows when each expert's rows begin a new one. All
-// lanes of a wave look at 64 experts at a time. of = -1: there are fewer.
+// Rows [begin, end) of expert e, or those behind the last one.
+__device__ inline void rowsOf(
+    const ProductShape& p,
+    int e,
+    int64_t& begin,
+    int64_t& end) {
+  begin = 0;
+  end = 0;
+  if (e <= p.experts) {
+    begin = clampOffset(p.offsets, e, p.m);
+    end = e < p.experts ? clampOffset(p.offsets, e + 1, p.m) : p.m;
+  }
+}
+
+__device__ inline int waveScan(int v) {
+  const int lane = threadIdx.x % kWave;
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int other = __shfl_up(v, o);
+    v += lane >= o ? other : 0;
+  }
+  return v;
+}
+
+// How many tiles of `size` rows there are when each expert's rows begin a
+// new one. All lanes of a wave look at 64 experts at a time.
+__device__ inline int countTiles(const ProductShape& p, int size) {
+  if (p.offsets == nullptr) {
+    return static_cast<int>((p.m + size - 1) / size);
+  }
+  int base = 0;
+  for (int from = 0; from <= p.experts; from += kWave) {
+    int64_t begin;
+    int64_t end;
+    rowsOf(p, from + static_cast<int>(threadIdx.x) % kWave, begin, end);
+    const int count =
+        end > begin ? static_cast<int>((end - begin + size - 1) / size) : 0;
+    base += uniform(__shfl(waveScan(count), kWave - 1));
+  }
+  return base;
+}
+
+// The tile-th of them. of = -1: there are fewer.
 __device__ inline RowTile findTile(
     const ProductShape& p,
-    int64_t tile,
+    int tile,
     int size) {
   if (p.offsets == nullptr) {
-    const int64_t begin = tile * size;
+    const int64_t begin = static_cast<int64_t>(tile) * size;
     const int64_t end = begin + size < p.m ? begin + size : p.m;
     return RowTile{begin < p.m ? 0 : -1, begin, end};
   }
-  const int lane = threadIdx.x % kWave;
-  int64_t base = 0;
+  int base = 0;
   for (int from = 0; from <= p.experts; from += kWave) {
-    const int e = from + lane;
-    int64_t begin = 0;
-    int64_t end = 0;
-    if (e <= p.experts) {
-      begin = clampOffset(p.offsets, e, p.m);
-      end = e < p.experts ? clampOffset(p.offsets, e + 1, p.m) : p.m;
-    }
+    int64_t begin;
+    int64_t end;
+    rowsOf(p, from + static_cast<int>(threadIdx.x) % kWave, begin, end);
     const int count =
         end > begin ? static_cast<int>((end - begin + size - 1) / size) : 0;
-    int sum = count;
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-      const int other = __shfl_up(sum, o);
-      sum += lane >= o ? other : 0;
-    }
-    const int64_t first = base + sum - count;
-    const uint64_t here =
-        __ballot(tile >= first && tile < first + count);
+    const int sum = waveScan(count);
+    const int first = base + sum - count;
+    const uint64_t here = __ballot(tile >= first && tile < first + count);
     if (here != 0) {
       const int at = __ffsll(static_cast<unsigned long long>(here)) - 1;
-      const int64_t from2 =
-          __shfl(begin + (tile - first) * size, at);
-      const int64_t to = __shfl(end, at);
+      const int64_t start = uniform(
+          __shfl(begin + static_cast<int64_t>(tile - first) * size, at));
+      const int64_t to = uniform(__shfl(end, at));
       return RowTile{
-          from + at, from2, from2 + size < to ? from2 + size : to};
+          uniform(from + at), start, start + size < to ? start + size : to};
     }
-    base += __shfl(sum, kWave - 1);
+    base += uniform(__shfl(sum, kWave - 1));
   }
   return RowTile{-1, 0, 0};
+}
+
+// Which tile this workgroup computes. Workgroups go to the card's eight dies
+// in turn, and each die has a cache of its own: a die takes tiles that lie
+// together, kBand rows of tiles at a time, column by column, so that the
+// workgroups that run at once on it read the same few bands of both operands.
+constexpr int kDies = 8;
+constexpr int kBand = 8;
+
+struct TileAt {
+  int m;
+  int n;
+};
+
+__device__ inline bool tileAt(int tilesM, int tilesN, TileAt& at) {
+  const int64_t total = static_cast<int64_t>(tilesM) * tilesN;
+  const int die = blockIdx.x % kDies;
+  const int64_t begin = total * die / kDies;
+  const int64_t id = begin + blockIdx.x / kDies;
+  if (id >= total * (die + 1) / kDies) {
+    return false;
+  }
+  const int band = static_cast<int>(id / (static_cast<int64_t>(kBand) * tilesN));
+  const int inBand =
+      static_cast<int>(id - static_cast<int64_t>(band) * kBand * tilesN);
+  const int left = tilesM - band * kBand;
+  const int height = left < kBand ? left : kBand;
+  at.m = band * kBand + inBand % height;
+  at.n = inBand / height;
+  return true;
+}
+
+unsigned gridOf(int64_t tiles) {
+  tiles = (tiles + kDies - 1) / kDies * kDies;
+  GA_ENFORCE_LE(tiles, INT32_MAX);
+  return static_cast<unsigned>(tiles);
 }
 
 // One operand of a product: rows of bytes, `rows` of them from `p` on.
@@ -305,49 +382,53 @@ struct Operand {
   bool whole; // rows begin on borders of 16 bytes
 };
 
-// Bytes k to k + 15 of a row, zeros in place of those outside [lo, hi).
-// Bytes that are masked may hold anything, NaN too, and are never used.
+// Bytes k to k + 15, zeros in place of those outside [lo, hi). What is
+// masked may hold anything, NaN too.
+__device__ inline uint4 maskOf(uint4 v, int64_t k, int64_t lo, int64_t hi) {
+  const int first = static_cast<int>(lo > k ? (lo - k < 16 ? lo - k : 16) : 0);
+  const int last = static_cast<int>(hi < k + 16 ? (hi > k ? hi - k : 0) : 16);
+  uint64_t w[2] = {static_cast<uint64_t>(v.y) << 32 | v.x,
+                   static_cast<uint64_t>(v.w) << 32 | v.z};
+#pragma unroll
+  for (int i = 0; i < 2; i++) {
+    const int f = first - i * 8;
+    const int l = last - i * 8;
+    w[i] = f > 7 || l < 1 ? 0
+                          : w[i] & ~0ull << (f > 0 ? f * 8 : 0) &
+            ~0ull >> (l < 8 ? 64 - l * 8 : 0);
+  }
+  return make_uint4(
+      static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[0] >> 32),
+      static_cast<uint32_t>(w[1]), static_cast<uint32_t>(w[1] >> 32));
+}
+
+// The same of a row in memory, of any alignment: none but its own bytes and
+// those of its operand are read.
 __device__ inline uint4 load16(
     const Operand& o,
     int64_t row,
     int64_t k,
     int64_t lo,
     int64_t hi) {
+  const int64_t at = row * o.stride + k;
   if (k >= hi || k + 16 <= lo) {
     return make_uint4(0, 0, 0, 0);
   }
-  const uint8_t* at = o.p + row * o.stride + k;
-  uint32_t w[4] = {0, 0, 0, 0};
-  const bool inside = row * o.stride + k + 16 <=
-      (o.rows - 1) * o.stride + o.inner;
-  if (o.whole && inside) {
-    const uint4 v = *reinterpret_cast<const uint4*>(at);
-    w[0] = v.x;
-    w[1] = v.y;
-    w[2] = v.z;
-    w[3] = v.w;
-    if (k < lo || k + 16 > hi) {
-      const int first = static_cast<int>(lo > k ? lo - k : 0);
-      const int last = static_cast<int>(hi < k + 16 ? hi - k : 16);
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-#pragma unroll
-        for (int c = 0; c < 4; c++) {
-          if (i * 4 + c < first || i * 4 + c >= last) {
-            w[i] &= ~(0xffu << (c * 8));
-          }
-        }
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < 16; i++) {
-      if (k + i >= lo && k + i < hi) {
-        w[i / 4] |= static_cast<uint32_t>(at[i]) << (i % 4 * 8);
-      }
-    }
+  if (o.whole && at + 16 <= (o.rows - 1) * o.stride + o.inner) {
+    return maskOf(*reinterpret_cast<const uint4*>(o.p + at), k, lo, hi);
   }
-  return make_uint4(w[0], w[1], w[2], w[3]);
+  uint64_t w[2] = {0, 0};
+  const int first = static_cast<int>(lo > k ? lo - k : 0);
+  const int last = static_cast<int>(hi < k + 16 ? hi - k : 16);
+#pragma unroll 1
+  for (int i = first; i < last; i++) {
+    const uint64_t byte = static_cast<uint64_t>(o.p[at + i]) << (i % 8 * 8);
+    w[0] |= i < 8 ? byte : 0;
+    w[1] |= i < 8 ? 0 : byte;
+  }
+  return make_uint4(
+      static_cast<uint32_t>(w[0]), static_cast<uint32_t>(w[0] >> 32),
+      static_cast<uint32_t>(w[1]), static_cast<uint32_t>(w[1] >> 32));
 }
 
 // Four results of a row, as one store where that is possible.
@@ -464,12 +545,19 @@ struct Job {
 };
 
 // A tile of results, TM x TN of the 32 x 32 instruction for each of WM x WN
-// waves, kQuant bytes of the inner dimension a step through LDS. The
+// waves, kQuant bytes of the inner dimension at a time through LDS. The
 // result's columns are the instruction's rows: a lane then holds four
 // adjacent columns of one row, and its row's scale is its own.
 //
-// LDS rows are 128 bytes; a row's 16-byte chunks are permuted by (row & 7),
-// so that eight rows' equal chunks lie in different banks.
+// LDS rows are 128 bytes, half of its 64 banks. A row's 16-byte chunks are
+// permuted by (row / 2) % 8, so that equal chunks of the 16 rows that one
+// cycle of a 16-byte read serves lie in 16 different places.
+constexpr int kChunks = kQuant / 16;
+
+__device__ inline int chunkOf(int row, int c) {
+  return c ^ (row >> 1 & 7);
+}
+
 template <int TM, int TN, int WM, int WN>
 struct Tile {
   static constexpr int kM = TM * WM * 32;
@@ -477,83 +565,201 @@ struct Tile {
   static constexpr int kThreads = WM * WN * kWave;
 };
 
+// Rows row0 to row0 + kRows - 1 of an operand on their way into LDS; those
+// from rowEnd on are copies of the last one, and their results are dropped.
 template <int kRows, int kThreads>
-__device__ inline void stage(
-    const Operand& o,
-    int64_t row0,
-    int64_t rowEnd,
-    int64_t k,
-    int64_t lo,
-    int64_t hi,
-    uint4* lds) {
+struct Stager {
+  static constexpr int kEach = kRows * kChunks / kThreads; // chunks a lane
+  const Operand& o;
+  int64_t row0;
+  int64_t rowEnd;
+  int64_t lo; // bytes of the inner dimension that count: [lo, hi)
+  int64_t hi;
+  bool direct;
+  __amdgpu_buffer_rsrc_t buffer;
+  int offset[kEach];
+
+  __device__ Stager(
+      const Operand& operand,
+      int64_t first,
+      int64_t end,
+      int64_t low,
+      int64_t high)
+      : o(operand), row0(first), rowEnd(end), lo(low), hi(high) {
+    // Offsets from row0 on are 32 bits wide.
+    const int64_t room = (o.rows - 1 - row0) * o.stride + o.inner;
+    direct = o.whole && o.stride <= (1 << 22) && o.inner < (1 << 28);
+    buffer = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(o.p + row0 * o.stride), 0,
+        static_cast<int>(room < (1ll << 31) - 1 ? room : (1ll << 31) - 1),
+        0x00027000);
+    // The wave writes 64 chunks to adjacent places: the permutation of a
+    // row's chunks is one of the lanes' addresses.
+    const int last = static_cast<int>(rowEnd - row0) - 1;
 #pragma unroll
-  for (int i = 0; i < kRows * 8 / kThreads; i++) {
-    const int chunk = i * kThreads + threadIdx.x;
-    const int row = chunk / 8;
-    const int c = chunk % 8;
-    const int64_t r = row0 + row < rowEnd ? row0 + row : rowEnd - 1;
-    lds[row * 8 + (c ^ (row & 7))] = load16(o, r, k + c * 16, lo, hi);
+    for (int i = 0; i < kEach; i++) {
+      const int chunk = i * kThreads + threadIdx.x;
+      const int row = chunk / kChunks;
+      const int c = chunkOf(row, chunk % kChunks);
+      offset[i] = (row < last ? row : last) * static_cast<int>(
+                      direct ? o.stride : 0) + c * 16;
+    }
   }
+
+  // Bytes k on, all of which count, straight into LDS: no registers and no
+  // wait until they are needed.
+  __device__ void loadDirect(int k, uint4* lds) const {
+    k = uniform(k);
+    const int wave = uniform(static_cast<int>(threadIdx.x / kWave));
+#pragma unroll
+    for (int i = 0; i < kEach; i++) {
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          buffer,
+          (__attribute__((address_space(3))) void*)(
+              lds + i * kThreads + wave * kWave),
+          16, offset[i], k, 0, 0);
+    }
+  }
+
+  // Zeros in place of what loadDirect brought and does not count.
+  __device__ void mask(int64_t k, uint4* lds) const {
+#pragma unroll 1
+    for (int i = 0; i < kEach; i++) {
+      const int chunk = i * kThreads + threadIdx.x;
+      const int c = chunkOf(chunk / kChunks, chunk % kChunks);
+      const int64_t at = k + c * 16;
+      if (at < lo || at + 16 > hi) {
+        lds[chunk] = maskOf(lds[chunk], at, lo, hi);
+      }
+    }
+  }
+
+  // The same for any bytes, through masks.
+  __device__ void loadMasked(int64_t k, uint4* lds) const {
+#pragma unroll 1
+    for (int i = 0; i < kEach; i++) {
+      const int chunk = i * kThreads + threadIdx.x;
+      const int row = chunk / kChunks;
+      const int c = chunkOf(row, chunk % kChunks);
+      const int64_t r = row0 + row < rowEnd ? row0 + row : rowEnd - 1;
+      lds[chunk] = load16(o, r, k + c * 16, lo, hi);
+    }
+  }
+};
+
+// The scales of a step's rows and columns, one a lane, on their way into
+// LDS. Bytes that are far apart take a cycle each to load: a wave's 64 lanes
+// fetch them once for the workgroup and not for every wave's fragments.
+template <bool kWeightGrad, typename T>
+struct ScaleStager {
+  static_assert(T::kM + T::kN <= T::kThreads, "one scale a lane");
+  static_assert(T::kM % kWave == 0, "a wave's scales are of one operand");
+  const uint8_t* p; // of the wave's operand
+  int64_t blocks;
+  int row;
+  int offset;
+  __amdgpu_buffer_rsrc_t buffer;
+
+  __device__ ScaleStager(const Job& job, int64_t n) : blocks(job.blocks) {
+    const int wave = uniform(static_cast<int>(threadIdx.x / kWave));
+    const bool ofA = wave < T::kM / kWave;
+    const int last = static_cast<int>(
+        ofA ? job.mEnd - 1 - job.m0
+            : (n - 1 - job.n0 < T::kN ? n - 1 - job.n0 : T::kN - 1));
+    row = static_cast<int>(threadIdx.x) - (ofA ? 0 : T::kM);
+    row = row < last ? row : last;
+    if (ofA) {
+      p = job.aScale + job.m0 * job.blocks;
+    } else if (kWeightGrad) {
+      p = job.bScale + job.n0 * job.blocks;
+    } else {
+      p = job.bScale + job.n0 / kQuant * job.blocks;
+      row /= kQuant;
+    }
+    offset = row * static_cast<int>(job.blocks);
+    buffer = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>(p), 0, 0x7fffffff, 0x00027000);
+  }
+
+  __device__ void loadDirect(int kb, int* ls) const {
+    const int wave = uniform(static_cast<int>(threadIdx.x / kWave));
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        buffer,
+        (__attribute__((address_space(3))) void*)(ls + wave * kWave), 1,
+        offset, uniform(kb), 0, 0);
+  }
+
+  __device__ void load(int kb, int* ls) const {
+    ls[threadIdx.x] = p[row * blocks + kb];
+  }
+};
+
+// The wave's loads into LDS but the last kLater have arrived, its reads are
+// done, and so have and are all other waves'. A plain barrier and not
+// __syncthreads(), which would wait for every load into LDS.
+template <int kLater>
+__device__ inline void arrived() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(kLater) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN>
-__device__ inline void
-computeTile(const Job& job, int64_t n, O* __restrict__ out) {
+struct Product {
   using T = Tile<TM, TN, WM, WN>;
-  constexpr bool kExact = std::is_same<O, float>::value;
-  __shared__ uint4 la[T::kM * 8];
-  __shared__ uint4 lb[T::kN * 8];
-  const int lane = threadIdx.x % kWave;
-  const int wave = threadIdx.x / kWave;
-  const int waveM = wave / WN * TM * 32;
-  const int waveN = wave % WN * TN * 32;
+  static constexpr bool kExact = std::is_same<O, float>::value;
+  const Job& job;
+  int64_t n;
+  int lane;
+  int waveM;
+  int waveN;
+  int sa[TM];
+  int sb[TN];
   Float16 acc[TN][TM];
+
+  __device__ Product(const Job& j, int64_t columns) : job(j), n(columns) {
+    const int wave = threadIdx.x / kWave;
+    lane = threadIdx.x % kWave;
+    waveM = wave / WN * TM * 32;
+    waveN = wave % WN * TN * 32;
 #pragma unroll
-  for (int i = 0; i < TN; i++) {
+    for (int i = 0; i < TN; i++) {
 #pragma unroll
-    for (int j = 0; j < TM; j++) {
-      acc[i][j] = 0.0f;
+      for (int k = 0; k < TM; k++) {
+        acc[i][k] = 0.0f;
+      }
     }
   }
-  const int64_t kb1 =
-      job.k1 > job.k0 ? (job.k1 + kQuant - 1) / kQuant : 0;
-  for (int64_t kb = job.k0 / kQuant; kb < kb1; kb++) {
-    __syncthreads();
-    stage<T::kM, T::kThreads>(
-        job.a, job.m0, job.mEnd, kb * kQuant, job.k0, job.k1, la);
-    stage<T::kN, T::kThreads>(
-        job.b, job.n0, n, kb * kQuant, job.k0, job.k1, lb);
-    int sa[TM];
-    int sb[TN];
+
+  __device__ void readScales(const int* ls) {
 #pragma unroll
     for (int j = 0; j < TM; j++) {
-      const int64_t m = job.m0 + waveM + j * 32 + lane % 32;
-      sa[j] =
-          job.aScale[(m < job.mEnd ? m : job.mEnd - 1) * job.blocks + kb];
+      sa[j] = ls[waveM + j * 32 + lane % 32];
     }
 #pragma unroll
     for (int i = 0; i < TN; i++) {
-      int64_t r = job.n0 + waveN + i * 32 + lane % 32;
-      r = r < n ? r : n - 1;
-      sb[i] = job.bScale[(kWeightGrad ? r : r / kQuant) * job.blocks + kb];
+      sb[i] = ls[T::kM + waveN + i * 32 + lane % 32];
     }
-    __syncthreads();
+  }
+
+  __device__ void step(const uint4* la, const uint4* lb, const int* ls) {
+    readScales(ls);
 #pragma unroll
-    for (int s = 0; s < 2; s++) {
+    for (int h = 0; h < 2; h++) {
       Fragment<kExact> fa[TM];
       Fragment<kExact> fb[TN];
-      const int c = s * 4 + lane / 32 * 2;
+      const int c = h * 4 + lane / 32 * 2;
 #pragma unroll
       for (int j = 0; j < TM; j++) {
         const int r = waveM + j * 32 + lane % 32;
-        fa[j].set(la[r * 8 + (c ^ (r & 7))],
-                  la[r * 8 + ((c + 1) ^ (r & 7))], sa[j]);
+        fa[j].set(la[r * kChunks + chunkOf(r, c)],
+                  la[r * kChunks + chunkOf(r, c + 1)], sa[j]);
       }
 #pragma unroll
       for (int i = 0; i < TN; i++) {
         const int r = waveN + i * 32 + lane % 32;
-        fb[i].set(lb[r * 8 + (c ^ (r & 7))],
-                  lb[r * 8 + ((c + 1) ^ (r & 7))], sb[i]);
+        fb[i].set(lb[r * kChunks + chunkOf(r, c)],
+                  lb[r * kChunks + chunkOf(r, c + 1)], sb[i]);
       }
 #pragma unroll
       for (int i = 0; i < TN; i++) {
@@ -564,6 +770,144 @@ computeTile(const Job& job, int64_t n, O* __restrict__ out) {
       }
     }
   }
+
+  // A ring of three stages of LDS: two are on their way while one is
+  // multiplied. Arrays of their own and not parts of one: the compiler sees
+  // that a read of one does not wait for loads into another.
+  __device__ void run() {
+    constexpr int kSizeA = T::kM * kChunks;
+    constexpr int kSizeB = T::kN * kChunks;
+    constexpr bool kThree = T::kM + T::kN <= 384;
+    __shared__ uint4 la0[kSizeA];
+    __shared__ uint4 lb0[kSizeB];
+    __shared__ uint4 la1[kSizeA];
+    __shared__ uint4 lb1[kSizeB];
+    __shared__ uint4 la2[kThree ? kSizeA : 1];
+    __shared__ uint4 lb2[kThree ? kSizeB : 1];
+    __shared__ int ls0[T::kThreads];
+    __shared__ int ls1[T::kThreads];
+    __shared__ int ls2[kThree ? T::kThreads : 1];
+    if (job.k1 <= job.k0) {
+      return;
+    }
+    using StageA = Stager<T::kM, T::kThreads>;
+    using StageB = Stager<T::kN, T::kThreads>;
+    const StageA a(job.a, job.m0, job.mEnd, job.k0, job.k1);
+    const StageB b(job.b, job.n0, n, job.k0, job.k1);
+    const ScaleStager<kWeightGrad, T> s(job, n);
+    const int first = uniform(static_cast<int>(job.k0 / kQuant));
+    const int last =
+        uniform(static_cast<int>((job.k1 + kQuant - 1) / kQuant));
+    // Blocks that lie within the rows, [first, direct), are loaded directly.
+    // An expert's first and last one may hold bytes of its neighbours: those
+    // come behind the others, [whole0, whole1), and are masked.
+    const int full = static_cast<int>(job.a.inner / kQuant);
+    const int direct = uniform(
+        a.direct && b.direct ? (last < full ? last : full) : first);
+    if (first < direct) {
+      int whole0 = uniform(
+          static_cast<int>((job.k0 + kQuant - 1) / kQuant));
+      int whole1 = uniform(static_cast<int>(job.k1 / kQuant));
+      whole1 = whole1 < direct ? whole1 : direct;
+      whole0 = whole0 < whole1 ? whole0 : whole1;
+      const int whole = whole1 - whole0;
+      const int total = direct - first;
+      // The t-th block in this order. Behind the last the loads go on with
+      // that one again: every step then has as many loads on their way.
+      const auto nth = [&](int t) {
+        t = t < total ? t : total - 1;
+        const int edge = first + t - whole;
+        return uniform(
+            t < whole ? whole0 + t : (edge < whole0 ? edge : edge + whole));
+      };
+      constexpr int kLater =
+          kThree ? StageA::kEach + StageB::kEach + 1 : 0;
+      const auto begin = [&](int t, uint4* la, uint4* lb, int* ls) {
+        const int kb = nth(t);
+        a.loadDirect(kb * kQuant, la);
+        b.loadDirect(kb * kQuant, lb);
+        s.loadDirect(kb, ls);
+      };
+      const auto rest = [&](int t, uint4* la, uint4* lb, const int* ls) {
+        if (t < total) {
+          if (t >= whole) {
+            const int64_t k = static_cast<int64_t>(nth(t)) * kQuant;
+            a.mask(k, la);
+            b.mask(k, lb);
+            arrived<63>();
+          }
+          step(la, lb, ls);
+        }
+      };
+      int t = 0;
+      begin(0, la0, lb0, ls0);
+      if constexpr (kThree) {
+        begin(1, la1, lb1, ls1);
+        for (; t + 2 < whole; t += 3) {
+          arrived<kLater>();
+          begin(t + 2, la2, lb2, ls2);
+          step(la0, lb0, ls0);
+          arrived<kLater>();
+          begin(t + 3, la0, lb0, ls0);
+          step(la1, lb1, ls1);
+          arrived<kLater>();
+          begin(t + 4, la1, lb1, ls1);
+          step(la2, lb2, ls2);
+        }
+        // at most two whole blocks and two edges are left
+        arrived<kLater>();
+        begin(t + 2, la2, lb2, ls2);
+        rest(t, la0, lb0, ls0);
+        arrived<kLater>();
+        begin(t + 3, la0, lb0, ls0);
+        rest(t + 1, la1, lb1, ls1);
+        arrived<0>();
+        rest(t + 2, la2, lb2, ls2);
+        rest(t + 3, la0, lb0, ls0);
+      } else {
+        for (; t + 1 < whole; t += 2) {
+          arrived<0>();
+          begin(t + 1, la1, lb1, ls1);
+          step(la0, lb0, ls0);
+          arrived<0>();
+          begin(t + 2, la0, lb0, ls0);
+          step(la1, lb1, ls1);
+        }
+        // at most one whole block and two edges are left
+        arrived<0>();
+        begin(t + 1, la1, lb1, ls1);
+        rest(t, la0, lb0, ls0);
+        arrived<0>();
+        begin(t + 2, la0, lb0, ls0);
+        rest(t + 1, la1, lb1, ls1);
+        arrived<0>();
+        rest(t + 2, la0, lb0, ls0);
+      }
+      arrived<0>();
+    }
+    // the block in which the rows end, and rows that begin on odd borders
+#pragma unroll 1
+    for (int kb = direct; kb < last; kb++) {
+      const int64_t k = static_cast<int64_t>(kb) * kQuant;
+      __syncthreads();
+      a.loadMasked(k, la0);
+      b.loadMasked(k, lb0);
+      s.load(kb, ls0);
+      __syncthreads();
+      step(la0, lb0, ls0);
+    }
+  }
+};
+
+template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN>
+__device__ inline void
+computeTile(const Job& job, int64_t n, O* __restrict__ out) {
+  Product<O, kWeightGrad, TM, TN, WM, WN> p(job, n);
+  p.run();
+  const int lane = p.lane;
+  const int waveM = p.waveM;
+  const int waveN = p.waveN;
+  const auto& acc = p.acc;
   const bool whole = n % 4 == 0;
 #pragma unroll
   for (int j = 0; j < TM; j++) {
@@ -586,10 +930,14 @@ computeTile(const Job& job, int64_t n, O* __restrict__ out) {
 }
 
 template <typename O, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * kWave) void
+__global__ __launch_bounds__(WM * WN * kWave, TM * TN > 8 ? 1 : 2) void
 matmulKernel(ProductShape p, O* __restrict__ out) {
   using T = Tile<TM, TN, WM, WN>;
-  const RowTile tile = findTile(p, blockIdx.x / p.tilesN, T::kM);
+  TileAt at;
+  if (!tileAt(countTiles(p, T::kM), p.tilesN, at)) {
+    return;
+  }
+  const RowTile tile = findTile(p, at.m, T::kM);
   if (tile.of < 0) {
     return;
   }
@@ -601,7 +949,7 @@ matmulKernel(ProductShape p, O* __restrict__ out) {
   job.blocks = (p.inner + kQuant - 1) / kQuant;
   job.m0 = tile.begin;
   job.mEnd = tile.end;
-  job.n0 = static_cast<int64_t>(blockIdx.x % p.tilesN) * T::kN;
+  job.n0 = static_cast<int64_t>(at.n) * T::kN;
   job.k0 = 0;
   job.k1 = p.inner;
   if (tile.of == p.experts) {
@@ -614,21 +962,24 @@ matmulKernel(ProductShape p, O* __restrict__ out) {
 }
 
 template <typename O, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * kWave) void
+__global__ __launch_bounds__(WM * WN * kWave, TM * TN > 8 ? 1 : 2) void
 weightGradKernel(ProductShape p, O* __restrict__ out) {
   using T = Tile<TM, TN, WM, WN>;
-  const int64_t tilesM = (p.m + T::kM - 1) / T::kM;
-  const int64_t rest = blockIdx.x / p.tilesN;
-  const int e = static_cast<int>(rest / tilesM);
+  const int tilesM = static_cast<int>((p.m + T::kM - 1) / T::kM);
+  TileAt at;
+  if (!tileAt(tilesM * p.experts, p.tilesN, at)) {
+    return;
+  }
+  const int e = at.m / tilesM;
   Job job;
   job.a = Operand{p.a, p.aStride, p.m, p.inner, p.aWhole};
   job.b = Operand{p.b, p.bStride, p.n, p.inner, p.bWhole};
   job.aScale = p.aScale;
   job.bScale = p.bScale;
   job.blocks = (p.inner + kQuant - 1) / kQuant;
-  job.m0 = rest % tilesM * T::kM;
+  job.m0 = static_cast<int64_t>(at.m % tilesM) * T::kM;
   job.mEnd = job.m0 + T::kM < p.m ? job.m0 + T::kM : p.m;
-  job.n0 = static_cast<int64_t>(blockIdx.x % p.tilesN) * T::kN;
+  job.n0 = static_cast<int64_t>(at.n) * T::kN;
   job.k0 = 0;
   job.k1 = p.inner;
   if (p.offsets != nullptr) {
@@ -637,6 +988,23 @@ weightGradKernel(ProductShape p, O* __restrict__ out) {
   }
   computeTile<O, true, TM, TN, WM, WN>(
       job, p.n, out + e * p.m * p.n);
+}
+
+// Large tiles read each operand's bytes less often, small ones are more of
+// them: the large ones are taken where each of 256 compute units has one.
+// Measured, in us, large and small: 8192 x 8192 x 8192 454 / 560, 4095 x
+// 8192 x 4096 136 / 164; 512 x 4096 x 4096 27 / 20, 1024 x 2048 x 2048 17 /
+// 12.
+using LargeTile = Tile<2, 2, 2, 4>;
+using SmallTile = Tile<2, 2, 2, 2>;
+constexpr int64_t kLargeFrom = 256;
+
+// Tiles of rows, at most: every expert's last one may be a part of one, and
+// so may that of the rows behind the last expert.
+template <typename T>
+int64_t tilesOf(T, const ProductShape& p, bool grouped) {
+  return grouped ? p.m / T::kM + std::min<int64_t>(p.experts + 1, p.m)
+                 : (p.m + T::kM - 1) / T::kM;
 }
 
 bool whole16(const void* p, int64_t stride) {
@@ -752,17 +1120,20 @@ void launchFp8Matmul(
     auto go = [&](auto kernel, auto tile) {
       using T = decltype(tile);
       p.tilesN = static_cast<int>((p.n + T::kN - 1) / T::kN);
-      // every expert's last tile may be a part of one, and so may the
-      // rows' behind the last expert
-      const int64_t tilesM = a.offsets == nullptr
-          ? (p.m + T::kM - 1) / T::kM
-          : p.m / T::kM + std::min<int64_t>(p.experts + 1, p.m);
-      GA_ENFORCE_LE(tilesM * p.tilesN, INT32_MAX);
+      const int64_t tilesM = tilesOf(tile, p, a.offsets != nullptr);
       hipLaunchKernelGGL(
-          kernel, dim3(static_cast<unsigned>(tilesM * p.tilesN)),
+          kernel, dim3(gridOf(tilesM * p.tilesN)),
           dim3(T::kThreads), 0, stream, p, static_cast<O*>(a.out));
     };
-    go(matmulKernel<O, 2, 2, 2, 2>, Tile<2, 2, 2, 2>{});
+    const auto tiles = [&](auto tile) {
+      return tilesOf(tile, p, a.offsets != nullptr) *
+          ((p.n + decltype(tile)::kN - 1) / decltype(tile)::kN);
+    };
+    if (tiles(LargeTile{}) >= kLargeFrom) {
+      go(matmulKernel<O, 2, 2, 2, 4>, LargeTile{});
+    } else {
+      go(matmulKernel<O, 2, 2, 2, 2>, SmallTile{});
+    }
   });
   GA_HIP_CHECK(hipGetLastError());
 }
@@ -796,12 +1167,17 @@ void launchFp8WeightGrad(
       p.tilesN = static_cast<int>((p.n + T::kN - 1) / T::kN);
       const int64_t tiles =
           (p.m + T::kM - 1) / T::kM * p.tilesN * p.experts;
-      GA_ENFORCE_LE(tiles, INT32_MAX);
       hipLaunchKernelGGL(
-          kernel, dim3(static_cast<unsigned>(tiles)), dim3(T::kThreads), 0,
+          kernel, dim3(gridOf(tiles)), dim3(T::kThreads), 0,
           stream, p, static_cast<O*>(a.out));
     };
-    go(weightGradKernel<O, 2, 2, 2, 2>, Tile<2, 2, 2, 2>{});
+    if ((p.m + LargeTile::kM - 1) / LargeTile::kM *
+            ((p.n + LargeTile::kN - 1) / LargeTile::kN) * p.experts >=
+        kLargeFrom) {
+      go(weightGradKernel<O, 2, 2, 2, 4>, LargeTile{});
+    } else {
+      go(weightGradKernel<O, 2, 2, 2, 2>, SmallTile{});
+    }
   });
   GA_HIP_CHECK(hipGetLastError());
 }

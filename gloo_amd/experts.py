@@ -23,7 +23,6 @@ from typing import NamedTuple, Optional
 
 import torch
 import torch.distributed as dist
-from torch.autograd.function import once_differentiable
 
 import gloo_amd as ga
 
@@ -50,29 +49,43 @@ class ExpertPlan(NamedTuple):
     offsets: torch.Tensor
 
 
-def _need(ok, what):
-    if not ok:
-        raise ValueError(what)
-
-
 def _tensor(t, name, dim, dtypes, like=None):
-    _need(isinstance(t, torch.Tensor), f"{name}: a tensor is needed")
-    _need(t.dim() == dim, f"{name}: {dim} dimensions are needed, got "
-          f"{tuple(t.shape)}")
-    _need(t.dtype in dtypes, f"{name}: one of {[str(d) for d in dtypes]} is "
-          f"needed, got {t.dtype}")
-    _need(like is None or t.device == like.device,
-          f"{name}: is on {t.device}, and others are on "
-          f"{like.device if like is not None else None}")
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{name}: a tensor is needed")
+    if t.dim() != dim:
+        raise ValueError(f"{name}: {dim} dimensions are needed, got "
+                         f"{tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise ValueError(f"{name}: one of {[str(d) for d in dtypes]} is "
+                         f"needed, got {t.dtype}")
+    if like is not None and t.device != like.device:
+        raise ValueError(f"{name}: is on {t.device}, and others are on "
+                         f"{like.device}")
 
 
 def _gpu(t, name):
     """The last check before a launch: the others hold on any device."""
-    _need(t.is_cuda, f"{name}: tensors on a GPU are needed, got {t.device}")
+    if not t.is_cuda:
+        raise ValueError(
+            f"{name}: tensors on a GPU are needed, got {t.device}")
 
 
 def _stream(t):
-    return torch.cuda.current_stream(t.device).cuda_stream
+    """The current stream's handle alone: a Stream object takes 2 us."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _differentiated(*tensors):
+    return torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in tensors)
+
+
+def _once():
+    """Backward passes run in grad mode only where they are to be
+    differentiated themselves."""
+    if torch.is_grad_enabled():
+        raise RuntimeError("the expert operators' gradients cannot be "
+                           "differentiated again (create_graph=True)")
 
 
 def _adjacent(t):
@@ -87,39 +100,41 @@ def _blocks(n):
 # ------------------------------------------------------------------- router
 
 
+def _route(logits, bias, k, score, groups, topk_groups, group_score,
+           renormalize, scale):
+    x = _adjacent(logits.detach())
+    tokens, experts = x.shape
+    weights = torch.empty(tokens, k, dtype=torch.float32, device=x.device)
+    ids = torch.empty(tokens, k, dtype=torch.int32, device=x.device)
+    _C.hip_expert_route(
+        x.data_ptr(), x.stride(0), _FLOATS[x.dtype],
+        0 if bias is None else bias.data_ptr(), tokens, experts, k, score,
+        groups, topk_groups, group_score, renormalize, scale,
+        weights.data_ptr(), ids.data_ptr(), x.get_device(), _stream(x))
+    return weights, ids
+
+
 class _Route(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, logits, bias, k, score, groups, topk_groups,
-                group_score, renormalize, scale):
-        tokens, experts = logits.shape
-        x = _adjacent(logits.detach())
-        weights = torch.empty(tokens, k, dtype=torch.float32,
-                              device=x.device)
-        ids = torch.empty(tokens, k, dtype=torch.int32, device=x.device)
-        _C.hip_expert_route(
-            x.data_ptr(), x.stride(0), _FLOATS[x.dtype],
-            0 if bias is None else bias.data_ptr(), tokens, experts, k,
-            score, groups, topk_groups, group_score, renormalize, scale,
-            weights.data_ptr(), ids.data_ptr(), x.get_device(), _stream(x))
+    def forward(ctx, logits, *options):
+        weights, ids = _route(logits, *options)
         ctx.mark_non_differentiable(ids)
         ctx.save_for_backward(logits, ids)
-        ctx.options = (score, renormalize, scale)
+        ctx.options = options
         return weights, ids
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad, _):
+        _once()
         logits, ids = ctx.saved_tensors
-        score, renormalize, scale = ctx.options
-        x = _adjacent(logits.detach())
-        grad = grad.contiguous()
+        _, k, score, _, _, _, renormalize, scale = ctx.options
+        x, grad = _adjacent(logits.detach()), grad.contiguous()
         dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
         _C.hip_expert_route_backward(
             x.data_ptr(), x.stride(0), _FLOATS[x.dtype], x.shape[0],
-            x.shape[1], ids.shape[1], score, renormalize, scale,
-            ids.data_ptr(), grad.data_ptr(), dx.data_ptr(), x.get_device(),
-            _stream(x))
-        return (dx,) + (None,) * 8
+            x.shape[1], k, score, renormalize, scale, ids.data_ptr(),
+            grad.data_ptr(), dx.data_ptr(), x.get_device(), _stream(x))
+        return dx, None, None, None, None, None, None, None, None
 
 
 def route(logits, k, *, score="softmax", bias=None, groups=1, topk_groups=1,
@@ -146,30 +161,41 @@ def route(logits, k, *, score="softmax", bias=None, groups=1, topk_groups=1,
     """
     _tensor(logits, "logits", 2, _FLOATS)
     tokens, experts = logits.shape
-    _need(1 <= experts <= _C.MAX_EXPERTS,
-          f"route: 1 to {_C.MAX_EXPERTS} experts, got {experts}")
-    _need(1 <= k <= min(experts, _C.MAX_TOPK),
-          f"route: k is 1 to {min(experts, _C.MAX_TOPK)} here, got {k}")
-    _need(score in ("softmax", "sigmoid"),
-          f"route: score is 'softmax' or 'sigmoid', got {score!r}")
-    _need(group_score in ("max", "top2"),
-          f"route: group_score is 'max' or 'top2', got {group_score!r}")
-    _need(1 <= groups <= _C.MAX_EXPERT_GROUPS and experts % groups == 0,
-          f"route: {experts} experts in {groups} equal groups (at most "
-          f"{_C.MAX_EXPERT_GROUPS})")
-    _need(1 <= topk_groups <= groups,
-          f"route: topk_groups is 1 to {groups}, got {topk_groups}")
-    _need(groups == 1 or k <= topk_groups * (experts // groups),
-          f"route: {topk_groups} groups of {experts // groups} experts hold "
-          f"fewer than k = {k}")
+    if not 1 <= experts <= _C.MAX_EXPERTS:
+        raise ValueError(
+            f"route: 1 to {_C.MAX_EXPERTS} experts, got {experts}")
+    if not 1 <= k <= min(experts, _C.MAX_TOPK):
+        raise ValueError(
+            f"route: k is 1 to {min(experts, _C.MAX_TOPK)} here, got {k}")
+    if score not in ("softmax", "sigmoid"):
+        raise ValueError(
+            f"route: score is 'softmax' or 'sigmoid', got {score!r}")
+    if group_score not in ("max", "top2"):
+        raise ValueError(
+            f"route: group_score is 'max' or 'top2', got {group_score!r}")
+    if not 1 <= groups <= _C.MAX_EXPERT_GROUPS or experts % groups != 0:
+        raise ValueError(
+            f"route: {experts} experts in {groups} equal groups (at most "
+            f"{_C.MAX_EXPERT_GROUPS})")
+    if not 1 <= topk_groups <= groups:
+        raise ValueError(
+            f"route: topk_groups is 1 to {groups}, got {topk_groups}")
+    if groups != 1 and k > topk_groups * (experts // groups):
+        raise ValueError(
+            f"route: {topk_groups} groups of {experts // groups} experts hold "
+            f"fewer than k = {k}")
     if bias is not None:
         _tensor(bias, "bias", 1, (torch.float32,), logits)
-        _need(bias.shape[0] == experts,
-              f"bias: {experts} values are needed, got {bias.shape[0]}")
+        if bias.shape[0] != experts:
+            raise ValueError(
+                f"bias: {experts} values are needed, got {bias.shape[0]}")
         bias = bias.detach().contiguous()
     _gpu(logits, "route")
-    return _Route.apply(logits, bias, k, score, groups, topk_groups,
-                        group_score, bool(renormalize), float(scale))
+    options = (bias, k, score, groups, topk_groups, group_score,
+               bool(renormalize), float(scale))
+    if _differentiated(logits):
+        return _Route.apply(logits, *options)
+    return _route(logits, *options)
 
 
 # ------------------------------------------------- plan, pack and combine
@@ -179,11 +205,13 @@ def plan(experts, num_experts):
     """Sorts token copies by expert (stable). experts [tokens, k] int32, as
     `route` gives them; numbers outside [0, num_experts) are no expert."""
     _tensor(experts, "experts", 2, (torch.int32,))
-    _need(1 <= num_experts <= _C.MAX_EXPERTS,
-          f"plan: 1 to {_C.MAX_EXPERTS} experts, got {num_experts}")
+    if not 1 <= num_experts <= _C.MAX_EXPERTS:
+        raise ValueError(
+            f"plan: 1 to {_C.MAX_EXPERTS} experts, got {num_experts}")
     ids = experts.contiguous()
     n = ids.numel()
-    _need(n < 2 ** 31, f"plan: fewer than 2^31 token copies, got {n}")
+    if n >= 2 ** 31:
+        raise ValueError(f"plan: fewer than 2^31 token copies, got {n}")
     _gpu(ids, "plan")
     dev = ids.device
     position = torch.empty(ids.shape, dtype=torch.int32, device=dev)
@@ -209,11 +237,13 @@ def _rows_args(position, hidden, dtype):
 def _check_plan(p, tokens, like):
     position = p.position
     _tensor(position, "plan.position", 2, (torch.int32,), like)
-    _need(position.is_contiguous(), "plan.position has to be contiguous")
-    _need(tokens is None or position.shape[0] == tokens,
-          f"the plan is for {position.shape[0]} tokens, got {tokens}")
-    _need(position.shape[1] > 0 and position.numel() < 2 ** 31,
-          f"plan.position: got {tuple(position.shape)}")
+    if not position.is_contiguous():
+        raise ValueError("plan.position has to be contiguous")
+    if tokens is not None and position.shape[0] != tokens:
+        raise ValueError(
+            f"the plan is for {position.shape[0]} tokens, got {tokens}")
+    if position.shape[1] <= 0 or position.numel() >= 2 ** 31:
+        raise ValueError(f"plan.position: got {tuple(position.shape)}")
     return position
 
 
@@ -249,8 +279,8 @@ class _Pack(torch.autograd.Function):
         return _pack(x.detach(), position)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
+        _once()
         position, = ctx.saved_tensors
         return _combine(grad, position, None), None
 
@@ -262,8 +292,8 @@ class _Combine(torch.autograd.Function):
         return _combine(rows.detach(), position, weights)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, grad):
+        _once()
         rows, position, weights = ctx.saved_tensors
         if weights is None:
             return _pack(grad, position), None, None
@@ -291,7 +321,9 @@ def pack(x, plan):
     _tensor(x, "x", 2, _FLOATS)
     position = _check_plan(plan, x.shape[0], x)
     _gpu(x, "pack")
-    return _Pack.apply(x, position)
+    if _differentiated(x):
+        return _Pack.apply(x, position)
+    return _pack(x.detach(), position)
 
 
 def pack_fp8(x, plan):
@@ -326,25 +358,28 @@ def combine(rows, plan, weights=None):
     Differentiable with respect to rows and weights."""
     _tensor(rows, "rows", 2, _FLOATS)
     position = _check_plan(plan, None, rows)
-    _need(rows.shape[0] == position.numel(),
-          f"rows: the plan has {position.numel()}, got {rows.shape[0]}")
+    if rows.shape[0] != position.numel():
+        raise ValueError(
+            f"rows: the plan has {position.numel()}, got {rows.shape[0]}")
     if weights is not None:
         _tensor(weights, "weights", 2, (torch.float32,), rows)
-        _need(weights.shape == position.shape,
-              f"weights: {tuple(position.shape)} is needed, got "
-              f"{tuple(weights.shape)}")
+        if weights.shape != position.shape:
+            raise ValueError(
+                f"weights: {tuple(position.shape)} is needed, got "
+                f"{tuple(weights.shape)}")
         weights = weights.contiguous()
     _gpu(rows, "combine")
-    return _Combine.apply(rows, position, weights)
+    if _differentiated(rows, weights):
+        return _Combine.apply(rows, position, weights)
+    return _combine(rows.detach(), position, weights)
 
 
 # ------------------------------------------------------------ 8-bit products
 
 
 def _no_gradient(name, *tensors):
-    _need(not (torch.is_grad_enabled()
-               and any(t.requires_grad for t in tensors)),
-          f"{name} has no gradient: detach() its inputs")
+    if _differentiated(*tensors):
+        raise ValueError(f"{name} has no gradient: detach() its inputs")
 
 
 def _fp8_rows(shape, width, device):
@@ -389,9 +424,10 @@ def quantize_fp8(x, tile=False):
 
 def _quantize(x, tile, q, stride, scales):
     x = x.detach()
-    _need(x.shape[1] <= 65535 * FP8_BLOCK,
-          f"quantize_fp8: at most {65535 * FP8_BLOCK} columns, got "
-          f"{x.shape[1]}")
+    if x.shape[1] > 65535 * FP8_BLOCK:
+        raise ValueError(
+            f"quantize_fp8: at most {65535 * FP8_BLOCK} columns, got "
+            f"{x.shape[1]}")
     if x.numel():
         _C.hip_quantize_fp8(
             x.data_ptr(), x.stride(0), x.stride(1), _FLOATS[x.dtype],
@@ -402,9 +438,9 @@ def _quantize(x, tile, q, stride, scales):
 def _fp8_operand(q, scale, name, dim, scale_shape, like=None):
     _tensor(q, name, dim, (FP8,), like)
     _tensor(scale, f"{name}_scale", dim, (FP8_SCALE,), q)
-    _need(tuple(scale.shape) == scale_shape,
-          f"{name}_scale: {scale_shape} is needed, got "
-          f"{tuple(scale.shape)}")
+    if tuple(scale.shape) != scale_shape:
+        raise ValueError(f"{name}_scale: {scale_shape} is needed, got "
+                         f"{tuple(scale.shape)}")
     return _adjacent(q), scale.contiguous()
 
 
@@ -412,9 +448,10 @@ def _offsets(offsets, experts, like):
     if offsets is None:
         return 0
     _tensor(offsets, "offsets", 1, (torch.int32,), like)
-    _need(offsets.shape[0] == experts + 1 and offsets.is_contiguous(),
-          f"offsets: {experts + 1} adjacent numbers are needed, got "
-          f"{tuple(offsets.shape)}")
+    if offsets.shape[0] != experts + 1 or not offsets.is_contiguous():
+        raise ValueError(
+            f"offsets: {experts + 1} adjacent numbers are needed, got "
+            f"{tuple(offsets.shape)}")
     return offsets.data_ptr()
 
 
@@ -430,18 +467,21 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
     offsets[e + 1] are multiplied by b[e]; rows behind the last expert's are
     zeros. The data gradient is the same product with the weights'
     transposed copy; `fp8_weight_grad` is the other one."""
-    _need(isinstance(a, torch.Tensor) and a.dim() == 2,
-          "a: a tensor of 2 dimensions is needed")
-    _need(isinstance(b, torch.Tensor)
-          and b.dim() == (2 if offsets is None else 3),
-          "b: [n, inner], or [experts, n, inner] with offsets")
-    _need(dtype in _FLOATS, f"fp8_matmul: cannot return {dtype}")
+    if not isinstance(a, torch.Tensor) or a.dim() != 2:
+        raise ValueError("a: a tensor of 2 dimensions is needed")
+    if (not isinstance(b, torch.Tensor)
+            or b.dim() != (2 if offsets is None else 3)):
+        raise ValueError("b: [n, inner], or [experts, n, inner] with offsets")
+    if dtype not in _FLOATS:
+        raise ValueError(f"fp8_matmul: cannot return {dtype}")
     rows, inner = a.shape
     n = b.shape[-2]
     experts = 1 if offsets is None else b.shape[0]
-    _need(b.shape[-1] == inner,
-          f"b: an inner dimension of {inner} is needed, got {b.shape[-1]}")
-    _need(n > 0 and experts > 0, f"b: got {tuple(b.shape)}")
+    if b.shape[-1] != inner:
+        raise ValueError(
+            f"b: an inner dimension of {inner} is needed, got {b.shape[-1]}")
+    if n <= 0 or experts <= 0:
+        raise ValueError(f"b: got {tuple(b.shape)}")
     a, a_scale = _fp8_operand(a, a_scale, "a", 2, (rows, _blocks(inner)))
     b, b_scale = _fp8_operand(
         b, b_scale, "b", b.dim(),
@@ -469,20 +509,24 @@ def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
     [experts + 1]) rows offsets[e] to offsets[e + 1] are expert e's, and the
     result is [experts, m, n], zeros for an expert without rows. Experts may
     begin anywhere: two of them can share a block and its scale."""
-    _need(isinstance(dy, torch.Tensor) and dy.dim() == 2
-          and isinstance(x, torch.Tensor) and x.dim() == 2,
-          "dy, x: tensors of 2 dimensions are needed")
-    _need(dtype in _FLOATS, f"fp8_weight_grad: cannot return {dtype}")
+    if (not isinstance(dy, torch.Tensor) or dy.dim() != 2 or not
+            isinstance(x, torch.Tensor) or x.dim() != 2):
+        raise ValueError("dy, x: tensors of 2 dimensions are needed")
+    if dtype not in _FLOATS:
+        raise ValueError(f"fp8_weight_grad: cannot return {dtype}")
     (m, rows), n = dy.shape, x.shape[0]
-    _need(x.shape[1] == rows, f"x: {rows} rows are needed, got {x.shape[1]}")
-    _need(m > 0 and n > 0, f"dy, x: got {tuple(dy.shape)}, "
-          f"{tuple(x.shape)}")
+    if x.shape[1] != rows:
+        raise ValueError(f"x: {rows} rows are needed, got {x.shape[1]}")
+    if m <= 0 or n <= 0:
+        raise ValueError(f"dy, x: got {tuple(dy.shape)}, "
+                         f"{tuple(x.shape)}")
     dy, dy_scale = _fp8_operand(dy, dy_scale, "dy", 2, (m, _blocks(rows)))
     x, x_scale = _fp8_operand(x, x_scale, "x", 2, (n, _blocks(rows)), dy)
     experts = 1
     if offsets is not None:
-        _need(isinstance(offsets, torch.Tensor) and offsets.dim() == 1
-              and offsets.shape[0] > 1, "offsets: [experts + 1] is needed")
+        if (not isinstance(offsets, torch.Tensor) or offsets.dim() != 1
+                or offsets.shape[0] <= 1):
+            raise ValueError("offsets: [experts + 1] is needed")
         experts = offsets.shape[0] - 1
     at = _offsets(offsets, experts, dy)
     _gpu(dy, "fp8_weight_grad")
