@@ -25,6 +25,7 @@ constexpr int kQuant = kFp8Block;
 using Int8 = int __attribute__((ext_vector_type(8)));
 using Bf16x2 = __bf16 __attribute__((ext_vector_type(2)));
 using Bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
+using Float4 = float __attribute__((ext_vector_type(4)));
 using Float16 = float __attribute__((ext_vector_type(16)));
 
 __device__ inline uint32_t absBits(float v) {
@@ -117,53 +118,73 @@ __global__ __launch_bounds__(256) void quantizeRowsKernel(
   }
 }
 
-// Any strides, and adjacent rows above all: a transposed matrix. 64 rows x
-// 128 columns go through LDS, so that lanes run along the rows for the loads
-// and along the columns for the stores.
-template <typename T>
+// Any strides, and adjacent rows above all: a transposed matrix. A workgroup
+// takes 256 bytes of each of 128 columns through LDS, so that lanes run along
+// the rows for loads and scales and along the columns for stores.
+template <typename T, bool kVec>
 __global__ __launch_bounds__(256) void quantizeColumnsKernel(
     const T* __restrict__ x,
     uint8_t* __restrict__ q,
     uint8_t* __restrict__ scales,
     QuantShape p) {
-  constexpr int kRows = 64;
-  __shared__ float tile[kRows][kQuant + 1];
+  constexpr int kSize = Vec16<T>::kSize;
+  constexpr int kRows = 16 * kSize; // 256 bytes
+  constexpr int kParts = 256 / kRows; // lanes that share a row
+  constexpr int kEach = kQuant / kParts; // columns of one of them
+  __shared__ Vec16<T> tile[kQuant][16];
+  __shared__ uint32_t most[kParts][kRows];
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
   const int64_t col0 = static_cast<int64_t>(blockIdx.y) * kQuant;
-  const int lane = threadIdx.x % kRows;
-  for (int c = threadIdx.x / kRows; c < kQuant; c += 256 / kRows) {
-    const int64_t row = row0 + lane;
+  const int chunk = threadIdx.x % 16;
+  const int64_t from = row0 + chunk * kSize;
+#pragma unroll
+  for (int i = 0; i < kQuant / 16; i++) {
+    const int c = i * 16 + threadIdx.x / 16;
     const int64_t col = col0 + c;
-    tile[lane][c] = row < p.rows && col < p.cols
-        ? toFloat(x[row * p.rowStride + col * p.colStride])
-        : 0.0f;
+    Vec16<T> v;
+    if (kVec && col < p.cols && from + kSize <= p.rows) {
+      v = *reinterpret_cast<const Vec16<T>*>(x + from + col * p.colStride);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kSize; j++) {
+        v.v[j] = col < p.cols && from + j < p.rows
+            ? x[(from + j) * p.rowStride + col * p.colStride]
+            : fromFloat<T>(0.0f);
+      }
+    }
+    tile[c][chunk] = v;
   }
   __syncthreads();
-  constexpr int kEach = 32; // four lanes a row
-  const int r = threadIdx.x / 4;
-  const int c0 = threadIdx.x % 4 * kEach;
+  const int r = threadIdx.x % kRows;
+  const int part = threadIdx.x / kRows;
   float v[kEach];
   uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < kEach; i++) {
-    v[i] = tile[r][c0 + i];
+    v[i] = toFloat(
+        reinterpret_cast<const T*>(tile[part * kEach + i])[r]);
     amax = maxBits(amax, absBits(v[i]));
   }
-  amax = laneMax<4>(amax);
+  most[part][r] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kParts; i++) {
+    amax = maxBits(amax, most[i][r]);
+  }
   const int64_t row = row0 + r;
   if (row >= p.rows) {
     return;
   }
   const uint32_t byte = fp8ScaleByte(amax);
   const float inv = fp8InverseScale(byte);
-  uint8_t* to = q + row * p.qStride + col0 + c0;
-  if (col0 + c0 + 16 <= p.qStride) {
-    storeFp8<16>(to, v, inv);
+  const int64_t at = col0 + part * kEach;
+#pragma unroll
+  for (int i = 0; i < kEach / 16; i++) {
+    if (at + i * 16 + 16 <= p.qStride) {
+      storeFp8<16>(q + row * p.qStride + at + i * 16, v + i * 16, inv);
+    }
   }
-  if (col0 + c0 + 32 <= p.qStride) {
-    storeFp8<16>(to + 16, v + 16, inv);
-  }
-  if (c0 == 0) {
+  if (part == 0) {
     scales[row * gridDim.y + blockIdx.y] = static_cast<uint8_t>(byte);
   }
 }
@@ -525,6 +546,26 @@ __device__ inline Float16 multiply(
 #pragma unroll
   for (int i = 0; i < 4; i++) {
     c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.v[i], b.v[i], c, 0, 0, 0);
+  }
+  return c;
+}
+
+// The same for 16 x 16 results, over 128 bytes.
+__device__ inline Float4 multiply(
+    const Fragment<false>& a,
+    const Fragment<false>& b,
+    Float4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+      a.v, b.v, c, 0, 0, 0, a.scale, 0, b.scale);
+}
+
+__device__ inline Float4 multiply(
+    const Fragment<true>& a,
+    const Fragment<true>& b,
+    Float4 c) {
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a.v[i], b.v[i], c, 0, 0, 0);
   }
   return c;
 }
@@ -930,7 +971,7 @@ computeTile(const Job& job, int64_t n, O* __restrict__ out) {
 }
 
 template <typename O, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * kWave, TM * TN > 8 ? 1 : 2) void
+__global__ __launch_bounds__(WM * WN * kWave, WM * WN / 4) void
 matmulKernel(ProductShape p, O* __restrict__ out) {
   using T = Tile<TM, TN, WM, WN>;
   TileAt at;
@@ -961,8 +1002,127 @@ matmulKernel(ProductShape p, O* __restrict__ out) {
   computeTile<O, false, TM, TN, WM, WN>(job, p.n, out);
 }
 
+// Few rows: the weights are read once and multiplied by few bytes, so what
+// counts is how many of them are on their way. A workgroup takes 16 columns;
+// its kWaves waves part the inner dimension, load their fragments from memory
+// as the 16 x 16 instruction wants them (16 rows of 128 bytes, whole lines)
+// and add their results up in LDS, in the order of the waves. An expert's
+// rows are taken MT * 16 at a time.
+template <typename O, int MT, int kWaves>
+__global__ __launch_bounds__(kWaves * kWave) void fewRowsKernel(
+    ProductShape p,
+    O* __restrict__ out) {
+  constexpr bool kExact = std::is_same<O, float>::value;
+  constexpr int kAhead = MT == 1 ? 4 : 2; // blocks on their way
+  __shared__ float4 partial[kWaves][MT][kWave];
+  const int lane = threadIdx.x % kWave;
+  const int wave = uniform(static_cast<int>(threadIdx.x / kWave));
+  const int64_t n0 = static_cast<int64_t>(blockIdx.x) * 16;
+  const int e = blockIdx.y;
+  int64_t begin = 0;
+  int64_t end = p.m;
+  if (p.offsets != nullptr) {
+    rowsOf(p, e, begin, end);
+  }
+  const bool whole = p.n % 4 == 0;
+  if (e == p.experts) { // rows behind the last expert's: zeros
+    const float zero[4] = {0, 0, 0, 0};
+    for (int64_t i = threadIdx.x; i < (end - begin) * 4;
+         i += kWaves * kWave) {
+      store4(out + (begin + i / 4) * p.n, n0 + i % 4 * 4, p.n, zero, whole);
+    }
+    return;
+  }
+  const int blocks = static_cast<int>((p.inner + kQuant - 1) / kQuant);
+  const Operand a{p.a, p.aStride, p.m, p.inner, true};
+  const Operand b{
+      p.b + e * p.bExpertStride, p.bStride, p.n, p.inner, true};
+  const int64_t n = n0 + lane % 16 < p.n ? n0 + lane % 16 : p.n - 1;
+  const uint8_t* bScale = p.bScale +
+      (e * ((p.n + kQuant - 1) / kQuant) + n0 / kQuant) * blocks;
+  const auto load = [&](const Operand& o, int64_t row, int kb, uint4* v) {
+    const int64_t k =
+        static_cast<int64_t>(kb) * kQuant + lane / 16 * 32;
+    if (static_cast<int64_t>(kb + 1) * kQuant <= p.inner) {
+      const auto* from =
+          reinterpret_cast<const uint4*>(o.p + row * o.stride + k);
+      v[0] = from[0];
+      v[1] = from[1];
+    } else {
+      v[0] = load16(o, row, k, 0, p.inner);
+      v[1] = load16(o, row, k + 16, 0, p.inner);
+    }
+  };
+  for (int64_t m0 = begin; m0 < end; m0 += MT * 16) {
+    Float4 acc[MT];
+    int64_t m[MT];
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+      acc[j] = 0.0f;
+      const int64_t r = m0 + j * 16 + lane % 16;
+      m[j] = r < end ? r : end - 1;
+    }
+    for (int kb0 = wave; kb0 < blocks; kb0 += kWaves * kAhead) {
+      uint4 vb[kAhead][2];
+      uint4 va[kAhead][MT][2];
+      int sb[kAhead];
+      int sa[kAhead][MT];
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        const int kb = kb0 + u * kWaves;
+        if (kb < blocks) {
+          load(b, n, kb, vb[u]);
+          sb[u] = bScale[kb];
+#pragma unroll
+          for (int j = 0; j < MT; j++) {
+            load(a, m[j], kb, va[u][j]);
+            sa[u][j] = p.aScale[m[j] * blocks + kb];
+          }
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; u++) {
+        if (kb0 + u * kWaves < blocks) {
+          Fragment<kExact> fb;
+          fb.set(vb[u][0], vb[u][1], sb[u]);
+#pragma unroll
+          for (int j = 0; j < MT; j++) {
+            Fragment<kExact> fa;
+            fa.set(va[u][j][0], va[u][j][1], sa[u][j]);
+            acc[j] = multiply(fb, fa, acc[j]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < MT; j++) {
+      partial[wave][j][lane] =
+          make_float4(acc[j][0], acc[j][1], acc[j][2], acc[j][3]);
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < MT * kWave; i += kWaves * kWave) {
+      const int j = i / kWave;
+      const int l = i % kWave;
+      float v[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        const float4 f = partial[w][j][l];
+        v[0] += f.x;
+        v[1] += f.y;
+        v[2] += f.z;
+        v[3] += f.w;
+      }
+      const int64_t r = m0 + j * 16 + l % 16;
+      if (r < end) {
+        store4(out + r * p.n, n0 + l / 16 * 4, p.n, v, whole);
+      }
+    }
+    __syncthreads();
+  }
+}
+
 template <typename O, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * kWave, TM * TN > 8 ? 1 : 2) void
+__global__ __launch_bounds__(WM * WN * kWave, WM * WN / 4) void
 weightGradKernel(ProductShape p, O* __restrict__ out) {
   using T = Tile<TM, TN, WM, WN>;
   const int tilesM = static_cast<int>((p.m + T::kM - 1) / T::kM);
@@ -1005,6 +1165,22 @@ template <typename T>
 int64_t tilesOf(T, const ProductShape& p, bool grouped) {
   return grouped ? p.m / T::kM + std::min<int64_t>(p.experts + 1, p.m)
                  : (p.m + T::kM - 1) / T::kM;
+}
+
+// How many times 16 rows fewRowsKernel takes at a time, 0 where tiles are
+// better. Measured for bf16 results, in us, this kernel and tiles: 1 row by
+// 8192 x 4096 8 / 17, 16 rows 12 / 18, 32 rows 17 / 17 (fp32 18 / 29); 64
+// rows by 2048 x 4096 15 / 18, by 8192 x 4096 30 / 18. Eight experts of 1024
+// x 4096 with 128 rows 14 / 18; 64 of 4096 x 2048 with 256 rows 155 / 110:
+// tiles take experts with few rows well if there are enough of them.
+int fewRows(const ProductShape& p, bool grouped, int64_t smallTiles) {
+  if (!p.aWhole || !p.bWhole) {
+    return 0;
+  }
+  if (grouped) {
+    return smallTiles < 256 && p.m <= 16 * p.experts ? 2 : 0;
+  }
+  return p.m <= 16 ? 1 : p.m <= 32 ? 2 : p.m <= 64 && p.n <= 4096 ? 4 : 0;
 }
 
 bool whole16(const void* p, int64_t stride) {
@@ -1079,12 +1255,20 @@ void launchQuantizeFp8(
             to, sc, p);
       }
     } else {
+      constexpr int kRows = 16 * Vec16<T>::kSize;
       const dim3 grid(
-          static_cast<unsigned>((rows + 63) / 64),
+          static_cast<unsigned>((rows + kRows - 1) / kRows),
           static_cast<unsigned>(blocks));
-      hipLaunchKernelGGL(
-          (quantizeColumnsKernel<T>), grid, dim3(256), 0, stream, from, to,
-          sc, p);
+      if (rowStride == 1 && aligned16(x) &&
+          colStride % Vec16<T>::kSize == 0) {
+        hipLaunchKernelGGL(
+            (quantizeColumnsKernel<T, true>), grid, dim3(256), 0, stream,
+            from, to, sc, p);
+      } else {
+        hipLaunchKernelGGL(
+            (quantizeColumnsKernel<T, false>), grid, dim3(256), 0, stream,
+            from, to, sc, p);
+      }
     }
   });
   GA_HIP_CHECK(hipGetLastError());
@@ -1129,6 +1313,36 @@ void launchFp8Matmul(
       return tilesOf(tile, p, a.offsets != nullptr) *
           ((p.n + decltype(tile)::kN - 1) / decltype(tile)::kN);
     };
+    const int few = fewRows(
+        p, a.offsets != nullptr, tiles(SmallTile{}));
+    if (few != 0) {
+      const auto goFew = [&](auto rows, auto waves) {
+        constexpr int kRows = decltype(rows)::value;
+        constexpr int kWaves = decltype(waves)::value;
+        const dim3 grid(
+            static_cast<unsigned>((p.n + 15) / 16),
+            a.offsets != nullptr ? p.experts + 1 : 1);
+        hipLaunchKernelGGL(
+            (fewRowsKernel<O, kRows, kWaves>), grid, dim3(kWaves * kWave), 0,
+            stream, p, static_cast<O*>(a.out));
+      };
+      // Eight waves where each still has four blocks.
+      const auto goWaves = [&](auto rows) {
+        if (p.inner >= 32 * kQuant) {
+          goFew(rows, std::integral_constant<int, 8>{});
+        } else {
+          goFew(rows, std::integral_constant<int, 4>{});
+        }
+      };
+      if (few == 1) {
+        goWaves(std::integral_constant<int, 1>{});
+      } else if (few == 2) {
+        goWaves(std::integral_constant<int, 2>{});
+      } else {
+        goWaves(std::integral_constant<int, 4>{});
+      }
+      return;
+    }
     if (tiles(LargeTile{}) >= kLargeFrom) {
       go(matmulKernel<O, 2, 2, 2, 4>, LargeTile{});
     } else {
