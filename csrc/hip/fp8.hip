@@ -599,8 +599,9 @@ __device__ inline int chunkOf(int row, int c) {
   return c ^ (row >> 1 & 7);
 }
 
-template <int TM, int TN, int WM, int WN>
+template <int TM, int TN, int WM, int WN, int kStagesOf = 3>
 struct Tile {
+  static constexpr int kStages = kStagesOf;
   static constexpr int kM = TM * WM * 32;
   static constexpr int kN = TN * WN * 32;
   static constexpr int kThreads = WM * WN * kWave;
@@ -745,9 +746,9 @@ __device__ inline void arrived() {
   asm volatile("" ::: "memory");
 }
 
-template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN>
+template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN, int S>
 struct Product {
-  using T = Tile<TM, TN, WM, WN>;
+  using T = Tile<TM, TN, WM, WN, S>;
   static constexpr bool kExact = std::is_same<O, float>::value;
   const Job& job;
   int64_t n;
@@ -812,13 +813,13 @@ struct Product {
     }
   }
 
-  // A ring of three stages of LDS: two are on their way while one is
-  // multiplied. Arrays of their own and not parts of one: the compiler sees
+  // A ring of three stages of LDS, two on their way while one is multiplied,
+  // or of two, one on its way. Arrays of their own and not parts of one: the compiler sees
   // that a read of one does not wait for loads into another.
   __device__ void run() {
     constexpr int kSizeA = T::kM * kChunks;
     constexpr int kSizeB = T::kN * kChunks;
-    constexpr bool kThree = T::kM + T::kN <= 384;
+    constexpr bool kThree = S == 3;
     __shared__ uint4 la0[kSizeA];
     __shared__ uint4 lb0[kSizeB];
     __shared__ uint4 la1[kSizeA];
@@ -940,10 +941,10 @@ struct Product {
   }
 };
 
-template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN>
+template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN, int S>
 __device__ inline void
 computeTile(const Job& job, int64_t n, O* __restrict__ out) {
-  Product<O, kWeightGrad, TM, TN, WM, WN> p(job, n);
+  Product<O, kWeightGrad, TM, TN, WM, WN, S> p(job, n);
   p.run();
   const int lane = p.lane;
   const int waveM = p.waveM;
@@ -970,10 +971,10 @@ computeTile(const Job& job, int64_t n, O* __restrict__ out) {
   }
 }
 
-template <typename O, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * kWave, WM * WN / 4) void
+template <typename O, int TM, int TN, int WM, int WN, int S = 3>
+__global__ __launch_bounds__(WM * WN * kWave, S == 3 ? WM * WN / 4 : 2) void
 matmulKernel(ProductShape p, O* __restrict__ out) {
-  using T = Tile<TM, TN, WM, WN>;
+  using T = Tile<TM, TN, WM, WN, S>;
   TileAt at;
   if (!tileAt(countTiles(p, T::kM), p.tilesN, at)) {
     return;
@@ -999,7 +1000,7 @@ matmulKernel(ProductShape p, O* __restrict__ out) {
     job.b.p += tile.of * p.bExpertStride;
     job.bScale += tile.of * ((p.n + kQuant - 1) / kQuant) * job.blocks;
   }
-  computeTile<O, false, TM, TN, WM, WN>(job, p.n, out);
+  computeTile<O, false, TM, TN, WM, WN, S>(job, p.n, out);
 }
 
 // Few rows: the weights are read once and multiplied by few bytes, so what
@@ -1121,10 +1122,10 @@ __global__ __launch_bounds__(kWaves * kWave) void fewRowsKernel(
   }
 }
 
-template <typename O, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM * WN * kWave, WM * WN / 4) void
+template <typename O, int TM, int TN, int WM, int WN, int S = 3>
+__global__ __launch_bounds__(WM * WN * kWave, S == 3 ? WM * WN / 4 : 2) void
 weightGradKernel(ProductShape p, O* __restrict__ out) {
-  using T = Tile<TM, TN, WM, WN>;
+  using T = Tile<TM, TN, WM, WN, S>;
   const int tilesM = static_cast<int>((p.m + T::kM - 1) / T::kM);
   TileAt at;
   if (!tileAt(tilesM * p.experts, p.tilesN, at)) {
@@ -1146,18 +1147,26 @@ weightGradKernel(ProductShape p, O* __restrict__ out) {
     job.k0 = clampOffset(p.offsets, e, p.inner);
     job.k1 = clampOffset(p.offsets, e + 1, p.inner);
   }
-  computeTile<O, true, TM, TN, WM, WN>(
+  computeTile<O, true, TM, TN, WM, WN, S>(
       job, p.n, out + e * p.m * p.n);
 }
 
 // Large tiles read each operand's bytes less often, small ones are more of
-// them: the large ones are taken where each of 256 compute units has one.
-// Measured, in us, large and small: 8192 x 8192 x 8192 454 / 560, 4095 x
-// 8192 x 4096 136 / 164; 512 x 4096 x 4096 27 / 20, 1024 x 2048 x 2048 17 /
-// 12.
+// them: the large ones are taken where most of 256 compute units have one.
+// Measured for bf16 results, in us, large and small: 8192 x 8192 x 8192 454 /
+// 560, 4095 x 8192 x 4096 136 / 164, eight experts 2048 x 2048 x 2048 (up to
+// 200 large tiles) 22 / 27; 512 x 4096 x 4096 27 / 20, 1024 x 2048 x 2048
+// 17 / 12.
 using LargeTile = Tile<2, 2, 2, 4>;
 using SmallTile = Tile<2, 2, 2, 2>;
-constexpr int64_t kLargeFrom = 256;
+constexpr int64_t kLargeFrom = 192;
+// A weight gradient of experts with few rows is done with a tile after a few
+// steps: two workgroups on a compute unit, with two stages of LDS each, store
+// and multiply at the same time. 16 experts, 16384 x 4096 x 2048 (about eight
+// steps): 388 us against 448 with the large tile for fp32 results, 288 / 351
+// for bf16; from some 30 steps on the large tile is ahead.
+using PairTile = Tile<2, 2, 2, 2, 2>;
+constexpr int kShort = 32;
 
 // Tiles of rows, at most: every expert's last one may be a part of one, and
 // so may that of the rows behind the last expert.
@@ -1385,9 +1394,11 @@ void launchFp8WeightGrad(
           kernel, dim3(gridOf(tiles)), dim3(T::kThreads), 0,
           stream, p, static_cast<O*>(a.out));
     };
-    if ((p.m + LargeTile::kM - 1) / LargeTile::kM *
-            ((p.n + LargeTile::kN - 1) / LargeTile::kN) * p.experts >=
-        kLargeFrom) {
+    const int64_t large = (p.m + LargeTile::kM - 1) / LargeTile::kM *
+        ((p.n + LargeTile::kN - 1) / LargeTile::kN) * p.experts;
+    if (large >= kLargeFrom && p.inner / p.experts < kShort * kQuant) {
+      go(weightGradKernel<O, 2, 2, 2, 2, 2>, PairTile{});
+    } else if (large >= kLargeFrom) {
       go(weightGradKernel<O, 2, 2, 2, 4>, LargeTile{});
     } else {
       go(weightGradKernel<O, 2, 2, 2, 2>, SmallTile{});
