@@ -214,12 +214,9 @@ def plan(experts, num_experts):
         raise ValueError(f"plan: fewer than 2^31 token copies, got {n}")
     _gpu(ids, "plan")
     dev = ids.device
-    position = torch.empty(ids.shape, dtype=torch.int32, device=dev)
-    # one allocation: the counts, then the offsets on a border of 16 bytes
-    start = (num_experts + 3) // 4 * 4
-    both = torch.empty(start + num_experts + 1, dtype=torch.int32,
-                       device=dev)
-    counts, offsets = both[:num_experts], both[start:]
+    position = torch.empty_like(ids)
+    counts = torch.empty(num_experts, dtype=torch.int32, device=dev)
+    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
     size = _C.hip_expert_plan_workspace(n, num_experts)
     work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _C.hip_expert_plan(
@@ -338,14 +335,14 @@ def pack_fp8(x, plan):
     x = _adjacent(x.detach())
     hidden, n = x.shape[1], position.numel()
     q, stride = _fp8_rows((n,), hidden, x.device)
-    scales = torch.empty(n, _blocks(hidden), dtype=torch.uint8,
+    scales = torch.empty(n, _blocks(hidden), dtype=FP8_SCALE,
                          device=x.device)
     if n and hidden:
         _C.hip_expert_pack_fp8(
             *_rows_args(position, hidden, x.dtype), x.data_ptr(),
             x.stride(0), q.data_ptr(), stride, scales.data_ptr(),
             x.get_device(), _stream(x))
-    return q, scales.view(FP8_SCALE)
+    return q, scales
 
 
 def combine(rows, plan, weights=None):
@@ -386,6 +383,8 @@ def _fp8_rows(shape, width, device):
     """Room for rows of `width` 8-bit values that begin on borders of 128
     bytes, so that products can load them whole."""
     stride = _blocks(width) * FP8_BLOCK
+    if stride == width:
+        return torch.empty(*shape, width, dtype=FP8, device=device), stride
     q = torch.empty(*shape, stride, dtype=torch.uint8, device=device)
     return q.view(FP8)[..., :width], stride
 
@@ -407,19 +406,19 @@ def quantize_fp8(x, tile=False):
         experts, rows, cols = x.shape
         q, stride = _fp8_rows((experts, rows), cols, x.device)
         scales = torch.empty(experts, _blocks(rows), _blocks(cols),
-                             dtype=torch.uint8, device=x.device)
+                             dtype=FP8_SCALE, device=x.device)
         for e in range(experts):
             _quantize(x[e], True, q[e], stride, scales[e])
-        return q, scales.view(FP8_SCALE)
+        return q, scales
     _tensor(x, "x", 2, _FLOATS)
     _no_gradient("quantize_fp8", x)
     _gpu(x, "quantize_fp8")
     rows, cols = x.shape
     q, stride = _fp8_rows((rows,), cols, x.device)
     scales = torch.empty(_blocks(rows) if tile else rows, _blocks(cols),
-                         dtype=torch.uint8, device=x.device)
+                         dtype=FP8_SCALE, device=x.device)
     _quantize(x, bool(tile), q, stride, scales)
-    return q, scales.view(FP8_SCALE)
+    return q, scales
 
 
 def _quantize(x, tile, q, stride, scales):
