@@ -357,7 +357,8 @@ class ProcessGroupGlooAmd(dist.ProcessGroup):
                 ga.alltoall(self._ctx, h_out.data_ptr(), h_in.data_ptr(),
                             per, _gdtype(inp), tag=tag)
             else:
-                row = inp.numel() // inp.shape[0] if inp.dim() > 0 else 1
+                # of the shape and not of the count: a rank may have no rows
+                row = inp.shape[1:].numel()
                 in_counts = [int(s) * row for s in input_split_sizes]
                 out_counts = [int(s) * row for s in output_split_sizes]
                 ga.alltoallv(self._ctx, h_out.data_ptr(), h_in.data_ptr(),
