@@ -536,3 +536,150 @@ def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
         x.stride(0), x_scale.data_ptr(), at, m, n, rows, experts,
         out.data_ptr(), _FLOATS[dtype], dy.get_device(), _stream(dy))
     return out
+
+
+# ------------------------------------------------------- over a process group
+
+
+def _alltoall(pg, rows, send, recv):
+    """Rows [sum(send), ...] to the ranks in turn; returns [sum(recv), ...]."""
+    out = rows.new_empty((sum(recv),) + rows.shape[1:])
+    if pg.size() == 1:
+        return out.copy_(rows)
+    pg.alltoall_base(out, rows.contiguous(), recv, send,
+                     dist.AllToAllOptions()).wait()
+    return out
+
+
+class _AllToAll(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, pg, rows, send, recv):
+        ctx.way = pg, send, recv
+        return _alltoall(pg, rows.detach(), send, recv)
+
+    @staticmethod
+    def backward(ctx, grad):
+        _once()
+        pg, send, recv = ctx.way
+        return None, _alltoall(pg, grad, recv, send), None, None
+
+
+class ExpertBatch(NamedTuple):
+    """What a rank's experts are given, and the way back.
+
+    rows [n, hidden]: the token copies for this rank's experts, from all
+        ranks, by expert; scales [n, ceil(hidden / 128)] with 8-bit rows.
+    offsets [experts of a rank + 1] int32: where each expert's rows begin.
+    """
+    rows: torch.Tensor
+    scales: Optional[torch.Tensor]
+    offsets: torch.Tensor
+    sent: ExpertPlan
+    received: ExpertPlan
+    send: list
+    recv: list
+
+
+class ExpertExchange:
+    """Token copies to the ranks that hold their experts, and back.
+
+        exchange = ExpertExchange(num_experts, group)
+        weights, ids = route(logits, k)
+        batch = exchange.dispatch(x, ids)
+        y = ...                       # of batch.rows, by batch.offsets
+        out = exchange.combine(y, batch, weights)
+
+    Rank r of `group` (a "glooamd" process group, the default one if None)
+    holds experts r * E / size to (r + 1) * E / size - 1. Each rank packs its
+    tokens by expert, the counts travel as a small alltoall of host tensors
+    (so that dispatch waits for the GPU once), the rows as one alltoall with
+    split sizes, and what arrives from the ranks is packed by expert again.
+    All ranks call both methods, ranks without tokens too. With bf16 rows and
+    the like the whole way is differentiable; with `fp8` the rows and their
+    scales travel in 8 bits.
+    """
+
+    def __init__(self, num_experts, group=None):
+        self._pg = group
+        if group is None:
+            self._pg = dist.distributed_c10d._get_default_group()
+        size = self._pg.size()
+        if num_experts < 1 or num_experts % size:
+            raise ValueError(f"ExpertExchange: {num_experts} experts over "
+                             f"{size} ranks")
+        if num_experts > _C.MAX_EXPERTS:
+            raise ValueError(f"ExpertExchange: at most {_C.MAX_EXPERTS} "
+                             f"experts, got {num_experts}")
+        self.num_experts = num_experts
+        self.local_experts = num_experts // size
+
+    def _counts(self, counts):
+        """Copies of each local expert that each rank sends: a host tensor
+        [size, local experts], and this rank's own counts like it."""
+        mine = counts.view(-1, self.local_experts)
+        theirs = _alltoall(self._pg, mine, [1] * len(mine), [1] * len(mine))
+        return mine, theirs
+
+    def dispatch(self, x, experts, fp8=False):
+        """x [tokens, hidden], experts [tokens, k] int32 (-1: none): an
+        ExpertBatch with this rank's experts' rows."""
+        _tensor(x, "x", 2, _FLOATS)
+        _tensor(experts, "experts", 2, (torch.int32,), x)
+        if experts.shape[0] != x.shape[0] or experts.shape[1] < 1:
+            raise ValueError(f"experts: one row a token, got "
+                             f"{tuple(experts.shape)} for {x.shape[0]}")
+        _gpu(x, "dispatch")
+        if fp8:
+            _no_gradient("dispatch(fp8=True)", x)
+        hidden = x.shape[1]
+        sent = plan(experts, self.num_experts)
+        mine, theirs = self._counts(sent.counts.cpu())
+        send, recv = mine.sum(1).tolist(), theirs.sum(1).tolist()
+        if fp8:
+            rows = _joined(*pack_fp8(x, sent))[:sum(send)]
+        else:
+            rows = pack(x, sent)[:sum(send)]
+        rows = _AllToAll.apply(self._pg, rows, send, recv)
+        # from each rank its rows for the first expert, the second ...
+        ids = torch.arange(self.local_experts, dtype=torch.int32)
+        ids = ids.repeat(len(theirs)).repeat_interleave(theirs.reshape(-1))
+        received = plan(ids.view(-1, 1).to(x.device), self.local_experts)
+        scales = None
+        if fp8:
+            rows = pack(rows.view(torch.float32), received)
+            rows, scales = _parted(rows.view(torch.uint8), hidden)
+        else:
+            rows = pack(rows, received)
+        return ExpertBatch(rows, scales, received.offsets, sent, received,
+                           send, recv)
+
+    def combine(self, rows, batch, weights=None):
+        """The experts' results for batch.rows (float32, float16 or
+        bfloat16) back to the tokens: their sum by `weights` [tokens, k]."""
+        _tensor(rows, "rows", 2, _FLOATS, batch.offsets)
+        if rows.shape[0] != sum(batch.recv):
+            raise ValueError(f"rows: the batch has {sum(batch.recv)}, got "
+                             f"{rows.shape[0]}")
+        rows = combine(rows, batch.received)  # one row each: a permutation
+        rows = _AllToAll.apply(self._pg, rows, batch.recv, batch.send)
+        none = batch.sent.position.numel() - rows.shape[0]
+        if none:  # places of copies for no expert
+            rows = torch.cat([rows, rows.new_zeros(none, rows.shape[1])])
+        return combine(rows, batch.sent, weights)
+
+
+def _joined(q, scales):
+    """8-bit rows and their scales as rows of bytes, 16 at a time."""
+    n, wide = q.shape[0], _blocks(q.shape[1]) * FP8_BLOCK
+    rest = (scales.shape[1] + 15) // 16 * 16
+    out = torch.zeros(n, wide + rest, dtype=torch.uint8, device=q.device)
+    out[:, :q.shape[1]] = q.view(torch.uint8)
+    out[:, wide:wide + scales.shape[1]] = scales.view(torch.uint8)
+    return out
+
+
+def _parted(rows, hidden):
+    blocks = _blocks(hidden)
+    wide = blocks * FP8_BLOCK
+    scales = rows[:, wide:wide + blocks].contiguous()
+    return rows[:, :hidden].view(FP8), scales.view(FP8_SCALE)

@@ -158,3 +158,53 @@ def test_launchers_check_for_themselves():
     with pytest.raises(ga.EnforceNotMet):
         ga._C.hip_fp8_weight_grad(0, 128, 0, 0, 128, 0, 0, 4, 0, 8, 1, 0, f,
                                   0, s)
+
+
+def test_exchange_of_rows_between_ranks():
+    """The row exchange of ExpertExchange on host tensors, its gradient and
+    the counts, over three ranks; one rank sends nothing."""
+    from test_pg import spawn_pg
+
+    table = [[2, 0, 3, 1, 0, 4], [0] * 6, [1, 1, 0, 0, 5, 0]]
+
+    def fn(pg, rank, size):
+        exchange = ex.ExpertExchange(6, pg)
+        assert exchange.local_experts == 2
+        mine, theirs = exchange._counts(
+            torch.tensor(table[rank], dtype=torch.int32))
+        assert mine.tolist() == [table[rank][i:i + 2] for i in (0, 2, 4)]
+        assert theirs.tolist() == [
+            table[r][2 * rank:2 * rank + 2] for r in range(size)]
+        send, recv = mine.sum(1).tolist(), theirs.sum(1).tolist()
+        rows = torch.arange(sum(send) * 3.0).view(-1, 3) + 1000 * rank
+        rows.requires_grad_()
+        out = ex._AllToAll.apply(pg, rows, send, recv)
+        expect = []
+        for r in range(size):
+            n = [sum(table[r][2 * d:2 * d + 2]) for d in range(size)]
+            all_rows = torch.arange(sum(n) * 3.0).view(-1, 3) + 1000 * r
+            expect.append(all_rows.split(n)[rank])
+        assert torch.equal(out.detach(), torch.cat(expect))
+        grad, = torch.autograd.grad(out, rows, 2 * out.detach())
+        assert torch.equal(grad, 2 * rows.detach())
+        return True
+
+    spawn_pg(3, fn)
+
+
+def test_exchange_refuses():
+    from test_pg import spawn_pg
+
+    def fn(pg, rank, size):
+        for experts in (0, 3, 1026):
+            with pytest.raises(ValueError):
+                ex.ExpertExchange(experts, pg)
+        exchange = ex.ExpertExchange(4, pg)
+        ids = torch.zeros(4, 2, dtype=torch.int32)
+        with pytest.raises(ValueError, match="one row a token"):
+            exchange.dispatch(torch.zeros(5, 8), ids)
+        with pytest.raises(ValueError, match="on a GPU"):
+            exchange.dispatch(torch.zeros(4, 8), ids)
+        return True
+
+    spawn_pg(2, fn)

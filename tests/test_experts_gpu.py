@@ -924,3 +924,48 @@ def test_same_results_every_time():
             out, (rows, w), torch.ones_like(out))
         first = first or got
         assert all(torch.equal(a, b) for a, b in zip(first, got))
+
+
+def test_exchange_over_processes():
+    """Three ranks of an expert-parallel layer, each a process, on one GPU."""
+    import os
+    import socket
+    import subprocess
+    import sys
+
+    with socket.socket() as s:
+        s.bind(("127.0.0.1", 0))
+        port = s.getsockname()[1]
+    worker = os.path.join(os.path.dirname(__file__), "expert_worker.py")
+    procs = [subprocess.Popen(
+        [sys.executable, worker, str(r), "3", str(port)],
+        stdout=subprocess.PIPE, stderr=subprocess.STDOUT) for r in range(3)]
+    try:
+        outs = [p.communicate(timeout=100)[0].decode() for p in procs]
+    finally:
+        for p in procs:
+            if p.poll() is None:
+                p.kill()
+    for p, out in zip(procs, outs):
+        assert p.returncode == 0 and "ALL OK" in out, out[-2000:]
+
+
+def test_exchange_of_one_rank():
+    """A group of one: the way there and back without a collective."""
+    from gloo_amd.pg import ProcessGroupGlooAmd
+
+    gen = torch.Generator().manual_seed(21)
+    exchange = ex.ExpertExchange(8, ProcessGroupGlooAmd(ga.HashStore(), 0, 1))
+    x = torch.randn(20, 64, generator=gen).cuda().requires_grad_()
+    ids = ids_of(20, 2, 8, gen, 0.2)
+    w = torch.rand(20, 2, generator=gen).cuda()
+    batch = exchange.dispatch(x, ids.cuda())
+    out = exchange.combine(batch.rows, batch, w)
+    real = (ids >= 0).double()
+    each = real * w.double().cpu()
+    ref = x.detach().double().cpu() * each.sum(1, keepdim=True)
+    assert ((out.detach().double().cpu() - ref).abs()
+            <= 4 * U * ref.abs() + 1e-30).all()
+    dx, = torch.autograd.grad(out, x, torch.ones_like(out))
+    assert ((dx.double().cpu() - each.sum(1, keepdim=True)).abs()
+            <= 4 * U * each.sum(1, keepdim=True) + 1e-30).all()
