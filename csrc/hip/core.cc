@@ -32,15 +32,20 @@ std::string gpuPCIBusID(int device) {
   return std::string(buf);
 }
 
-HipStream::HipStream(int device) : device_(device) {
+HipStream::HipStream(int device, bool highPriority) : device_(device) {
   if (device_ >= 0) {
     GA_HIP_CHECK(hipSetDevice(device_));
   } else {
     GA_HIP_CHECK(hipGetDevice(&device_));
   }
-  // Default priority: work on streams of different priorities can stop
-  // making progress on this platform.
-  GA_HIP_CHECK(hipStreamCreateWithFlags(&stream_, hipStreamNonBlocking));
+  if (highPriority) {
+    int least = 0, greatest = 0;
+    GA_HIP_CHECK(hipDeviceGetStreamPriorityRange(&least, &greatest));
+    GA_HIP_CHECK(hipStreamCreateWithPriority(
+        &stream_, hipStreamNonBlocking, greatest));
+  } else {
+    GA_HIP_CHECK(hipStreamCreateWithFlags(&stream_, hipStreamNonBlocking));
+  }
   GA_HIP_CHECK(hipEventCreateWithFlags(&event_, hipEventDisableTiming));
 }
 
@@ -119,7 +124,9 @@ HipStream* pooledStream(const void* key, int device, int idx) {
       it = pool.emplace(k, std::move(fl.back())).first;
       fl.pop_back();
     } else {
-      it = pool.emplace(k, std::make_unique<HipStream>(device)).first;
+      it = pool.emplace(k, std::make_unique<HipStream>(
+                               device, /*highPriority=*/idx == 0))
+               .first;
     }
   }
   return it->second.get();

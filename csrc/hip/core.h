@@ -45,7 +45,7 @@ std::string gpuPCIBusID(int device);
 
 class HipStream {
  public:
-  explicit HipStream(int device = -1);
+  explicit HipStream(int device = -1, bool highPriority = false);
   ~HipStream();
   HipStream(const HipStream&) = delete;
   HipStream(HipStream&& o) noexcept;
@@ -71,7 +71,7 @@ class HipStream {
 // process+device; streams beyond that SHARE a queue, and a doorbell
 // spin kernel then head-of-line-blocks whatever shares its queue —
 // instant deadlock for flag-wait protocols. Capping each communicator
-// at 8 pooled streams (all of default priority) keeps every stream on
+// at 8 pooled streams (index 0 = high priority) keeps every stream on
 // its own hardware queue. Pool key: one per (communicator, device) —
 // different algorithm objects of one communicator intentionally reuse
 // the same streams (collectives on a communicator are serialized).
