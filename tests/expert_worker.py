@@ -1,4 +1,4 @@
-"""One rank of an expert-parallel layer on cuda:0 (see test_experts_gpu.py):
+"""One rank of an expert-parallel layer on cuda:0 (see test_gpu_experts.py):
 ExpertExchange over init_process_group("glooamd") against the same layer
 computed in this process alone."""
 import os

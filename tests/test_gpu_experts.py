@@ -4,6 +4,10 @@ implementations in 64 bits.
 Tolerances count roundings: one to a type t is off by at most
 finfo(t).eps / 2 of the value, a sum of n terms in 32 bits by n * 2^-24 of
 the sum of the terms' absolute values.
+
+These tests create streams, and are named so that they run behind test_gpu.py:
+its tests of two ranks in one process need hardware queues that no other
+stream of the process shares (docs/stability.md).
 """
 import math
 
