@@ -12,6 +12,7 @@
 //   gloo_amd_bench --size N --rank R [--store-file DIR | --store-tcp
 //   HOST:PORT] --benchmark allreduce_ring_chunked --elements -1
 //   [--gpu] [--half-precision] [--iteration-time-ms 2000]
+#include <cstdlib>
 #include <getopt.h>
 
 #include <thread>
@@ -542,7 +543,10 @@ void runOne(
 
 int main(int argc, char** argv) {
   // One HW queue per pooled stream (see csrc/hip/core.h pooledStream).
-  setenv("GPU_MAX_HW_QUEUES", "8", 0);
+  const char* queues = getenv("GPU_MAX_HW_QUEUES");
+  if (queues == nullptr || atoi(queues) < 8) {
+    setenv("GPU_MAX_HW_QUEUES", "8", 1);
+  }
   Options o = parse(argc, argv);
   if (o.benchmark.rfind("hip_", 0) == 0) {
     o.gpu = true; // hip_* benchmarks imply the device path

@@ -10,8 +10,20 @@ import os as _os
 
 # 8 hardware queues per process so each pooled stream owns one (the
 # ROCm default of 4 would multiplex streams onto shared queues, where a
-# doorbell spin kernel head-of-line-blocks the stream behind it).
-_os.environ.setdefault("GPU_MAX_HW_QUEUES", "8")
+# doorbell spin kernel head-of-line-blocks the stream behind it). An
+# environment that asks for fewer (launchers spell the default of 4 out) is
+# overruled: with 4 the engines of three ranks in a process can wait for each
+# other for good. HIP reads the variable at its first call.
+def _need_queues(least=8):
+    try:
+        have = int(_os.environ.get("GPU_MAX_HW_QUEUES", "0"))
+    except ValueError:
+        have = 0
+    if have < least:
+        _os.environ["GPU_MAX_HW_QUEUES"] = str(least)
+
+
+_need_queues()
 
 # Load torch (and its bundled HIP runtime) BEFORE our extension: _C's
 # libamdhip64.so.7 dependency then resolves by SONAME onto torch's
