@@ -1031,7 +1031,7 @@ RowsShape checkRows(const ExpertRowsArgs& a) {
   GA_ENFORCE_GT(a.k, 0);
   GA_ENFORCE_GT(a.hidden, 0);
   GA_ENFORCE_LE(a.tokens, INT32_MAX / a.k);
-  GA_ENFORCE_LE(a.hidden, 1 << 24);
+  GA_ENFORCE_LE(a.hidden, 1 << 23);
   return RowsShape{a.tokens, a.hidden, a.tokens * a.k, a.k};
 }
 

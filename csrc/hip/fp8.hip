@@ -599,9 +599,8 @@ __device__ inline int chunkOf(int row, int c) {
   return c ^ (row >> 1 & 7);
 }
 
-template <int TM, int TN, int WM, int WN, int kStagesOf = 3>
+template <int TM, int TN, int WM, int WN>
 struct Tile {
-  static constexpr int kStages = kStagesOf;
   static constexpr int kM = TM * WM * 32;
   static constexpr int kN = TN * WN * 32;
   static constexpr int kThreads = WM * WN * kWave;
@@ -748,7 +747,7 @@ __device__ inline void arrived() {
 
 template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN, int S>
 struct Product {
-  using T = Tile<TM, TN, WM, WN, S>;
+  using T = Tile<TM, TN, WM, WN>;
   static constexpr bool kExact = std::is_same<O, float>::value;
   const Job& job;
   int64_t n;
@@ -974,7 +973,7 @@ computeTile(const Job& job, int64_t n, O* __restrict__ out) {
 template <typename O, int TM, int TN, int WM, int WN, int S = 3>
 __global__ __launch_bounds__(WM * WN * kWave, S == 3 ? WM * WN / 4 : 2) void
 matmulKernel(ProductShape p, O* __restrict__ out) {
-  using T = Tile<TM, TN, WM, WN, S>;
+  using T = Tile<TM, TN, WM, WN>;
   TileAt at;
   if (!tileAt(countTiles(p, T::kM), p.tilesN, at)) {
     return;
@@ -1125,7 +1124,7 @@ __global__ __launch_bounds__(kWaves * kWave) void fewRowsKernel(
 template <typename O, int TM, int TN, int WM, int WN, int S = 3>
 __global__ __launch_bounds__(WM * WN * kWave, S == 3 ? WM * WN / 4 : 2) void
 weightGradKernel(ProductShape p, O* __restrict__ out) {
-  using T = Tile<TM, TN, WM, WN, S>;
+  using T = Tile<TM, TN, WM, WN>;
   const int tilesM = static_cast<int>((p.m + T::kM - 1) / T::kM);
   TileAt at;
   if (!tileAt(tilesM * p.experts, p.tilesN, at)) {
@@ -1161,11 +1160,10 @@ using LargeTile = Tile<2, 2, 2, 4>;
 using SmallTile = Tile<2, 2, 2, 2>;
 constexpr int64_t kLargeFrom = 192;
 // A weight gradient of experts with few rows is done with a tile after a few
-// steps: two workgroups on a compute unit, with two stages of LDS each, store
-// and multiply at the same time. 16 experts, 16384 x 4096 x 2048 (about eight
+// steps: two workgroups with small tiles on a compute unit, with two stages of
+// LDS each, store and multiply at the same time. 16 experts, 16384 x 4096 x 2048 (about eight
 // steps): 388 us against 448 with the large tile for fp32 results, 288 / 351
 // for bf16; from some 30 steps on the large tile is ahead.
-using PairTile = Tile<2, 2, 2, 2, 2>;
 constexpr int kShort = 32;
 
 // Tiles of rows, at most: every expert's last one may be a part of one, and
@@ -1204,6 +1202,7 @@ void checkProduct(const ProductShape& p) {
   GA_ENFORCE_LE(p.n, INT32_MAX);
   GA_ENFORCE_LE(p.inner, INT32_MAX);
   GA_ENFORCE_GT(p.experts, 0);
+  GA_ENFORCE_LT(p.experts, 65535);
   GA_ENFORCE_GE(p.aStride, 0);
   GA_ENFORCE_GE(p.bStride, 0);
 }
@@ -1397,7 +1396,7 @@ void launchFp8WeightGrad(
     const int64_t large = (p.m + LargeTile::kM - 1) / LargeTile::kM *
         ((p.n + LargeTile::kN - 1) / LargeTile::kN) * p.experts;
     if (large >= kLargeFrom && p.inner / p.experts < kShort * kQuant) {
-      go(weightGradKernel<O, 2, 2, 2, 2, 2>, PairTile{});
+      go(weightGradKernel<O, 2, 2, 2, 2, 2>, SmallTile{});
     } else if (large >= kLargeFrom) {
       go(weightGradKernel<O, 2, 2, 2, 4>, LargeTile{});
     } else {

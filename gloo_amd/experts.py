@@ -152,9 +152,9 @@ def route(logits, k, *, score="softmax", bias=None, groups=1, topk_groups=1,
     weight is its score, divided by the sum of the chosen ones' where
     `renormalize` is set, times `scale`.
 
-    An expert whose logit is -inf or NaN is never chosen: where a token has
-    fewer experts than k, the others are -1, with weight 0. +inf counts as
-    the largest float32.
+    An expert whose logit or bias is -inf or NaN is never chosen: where a
+    token has fewer experts than k, the others are -1, with weight 0. A logit
+    of +inf counts as the largest float32.
 
     Returns (weights [tokens, k] float32, experts [tokens, k] int32). The
     weights are differentiable with respect to the logits.
@@ -443,6 +443,12 @@ def _fp8_operand(q, scale, name, dim, scale_shape, like=None):
     return _adjacent(q), scale.contiguous()
 
 
+def _pitch(q):
+    """Bytes from one row to the next; a single row has none, whatever its
+    stride says, and begins where the tensor does."""
+    return q.stride(-2) if q.shape[-2] > 1 else 0
+
+
 def _offsets(offsets, experts, like):
     if offsets is None:
         return 0
@@ -490,8 +496,8 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
     out = torch.empty(rows, n, dtype=dtype, device=a.device)
     if rows:
         _C.hip_fp8_matmul(
-            a.data_ptr(), a.stride(0), a_scale.data_ptr(), b.data_ptr(),
-            b.stride(-2), 0 if offsets is None else b.stride(0),
+            a.data_ptr(), _pitch(a), a_scale.data_ptr(), b.data_ptr(),
+            _pitch(b), 0 if offsets is None else b.stride(0),
             b_scale.data_ptr(), at, rows, n, inner, experts, out.data_ptr(),
             _FLOATS[dtype], a.get_device(), _stream(a))
     return out
@@ -532,8 +538,8 @@ def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
     out = torch.empty((m, n) if offsets is None else (experts, m, n),
                       dtype=dtype, device=dy.device)
     _C.hip_fp8_weight_grad(
-        dy.data_ptr(), dy.stride(0), dy_scale.data_ptr(), x.data_ptr(),
-        x.stride(0), x_scale.data_ptr(), at, m, n, rows, experts,
+        dy.data_ptr(), _pitch(dy), dy_scale.data_ptr(), x.data_ptr(),
+        _pitch(x), x_scale.data_ptr(), at, m, n, rows, experts,
         out.data_ptr(), _FLOATS[dtype], dy.get_device(), _stream(dy))
     return out
 

@@ -752,6 +752,46 @@ def test_products_keep_nan_in_its_row():
     assert torch.isnan(got[1]).all()
 
 
+def test_weight_grad_of_neighbours_with_nan():
+    """The same where an expert's first and last blocks are loaded whole."""
+    gen = torch.Generator().manual_seed(5)
+    at = [0, 200, 330, 700]
+    dy, sy = operand((130, 700), (130, 6), gen)
+    x, sx = operand((70, 700), (70, 6), gen)
+    for t in (dy, x):
+        t.view(torch.uint8)[:, 200:330] = 0x7f
+    off = torch.tensor(at, dtype=torch.int32).cuda()
+    for out in (torch.float32, torch.bfloat16):
+        got = ex.fp8_weight_grad(
+            dy.cuda(), sy.cuda(), x.cuda(), sx.cuda(), offsets=off, dtype=out)
+        assert torch.isnan(got[1]).all()
+        for e in (0, 2):
+            i, j = at[e], at[e + 1]
+            close(got[e], (dy.double() * wide_scale(sy, 700, 1))[:, i:j],
+                  (x.double() * wide_scale(sx, 700, 1))[:, i:j])
+
+
+def test_single_rows_of_any_stride():
+    gen = torch.Generator().manual_seed(6)
+    a, sa = operand((1, 512), (1, 4), gen)
+    b, sb = operand((64, 512), (1, 4), gen)
+    ref = ex.fp8_matmul(a.cuda(), sa.cuda(), b.cuda(), sb.cuda())
+    odd = a.cuda().as_strided((1, 512), (7, 1))
+    assert torch.equal(ex.fp8_matmul(odd, sa.cuda(), b.cuda(), sb.cuda()),
+                       ref)
+
+
+def test_gradients_of_gradients_are_refused():
+    p = ex.plan(torch.zeros(2, 1, dtype=torch.int32, device="cuda"), 1)
+    x = torch.randn(2, 8, device="cuda", requires_grad=True)
+    w = torch.ones(2, 1, device="cuda", requires_grad=True)
+    z = torch.randn(2, 4, device="cuda", requires_grad=True)
+    for out, leaf in ((ex.pack(x, p), x), (ex.combine(x, p, w), w),
+                      (ex.route(z, 2, renormalize=False)[0], z)):
+        with pytest.raises(RuntimeError, match="differentiated again"):
+            torch.autograd.grad(out.sum(), leaf, create_graph=True)
+
+
 def test_offsets_that_are_wrong_stay_inside():
     """Offsets are read on the device: wrong ones give wrong results, and
     touch nothing outside the tensors."""
