@@ -1151,14 +1151,22 @@ weightGradKernel(ProductShape p, O* __restrict__ out) {
 }
 
 // Large tiles read each operand's bytes less often, small ones are more of
-// them: the large ones are taken where most of 256 compute units have one.
-// Measured for bf16 results, in us, large and small: 8192 x 8192 x 8192 454 /
-// 560, 4095 x 8192 x 4096 136 / 164, eight experts 2048 x 2048 x 2048 (up to
-// 200 large tiles) 22 / 27; 512 x 4096 x 4096 27 / 20, 1024 x 2048 x 2048
-// 17 / 12.
+// them: the largest is taken of which there are enough, most of the 256
+// compute units having one. Measured for bf16 results, in us:
+//                       128 x 256  128 x 128  64 x 128  64 x 64
+//   8192 x 8192 x 8192     454       560
+//   1024 x 4096 x 4096                23.5      24.7     30.3
+//    512 x 4096 x 4096      27        19.7      15.0     16.0
+//    256 x 4096 x 4096                18.9      12.3      9.8
+//   1024 x 2048 x 2048      17        13.1      10.2     11.0
+// weight gradient of 16384 rows, 2048 x 2048 and 1024 x 1024:
+//                          137        97.5     114.9    140.1
+//                                     87.2      58.1     39.6
 using LargeTile = Tile<2, 2, 2, 4>;
 using SmallTile = Tile<2, 2, 2, 2>;
-constexpr int64_t kLargeFrom = 192;
+using HalfTile = Tile<1, 2, 2, 2>;
+using QuarterTile = Tile<1, 1, 2, 2>;
+constexpr int64_t kEnough = 192;
 // A weight gradient of experts with few rows is done with a tile after a few
 // steps: two workgroups with small tiles on a compute unit, with two stages of
 // LDS each, store and multiply at the same time. 16 experts, 16384 x 4096 x 2048 (about eight
@@ -1175,19 +1183,22 @@ int64_t tilesOf(T, const ProductShape& p, bool grouped) {
 }
 
 // How many times 16 rows fewRowsKernel takes at a time, 0 where tiles are
-// better. Measured for bf16 results, in us, this kernel and tiles: 1 row by
-// 8192 x 4096 8 / 17, 16 rows 12 / 18, 32 rows 17 / 17 (fp32 18 / 29); 64
-// rows by 2048 x 4096 15 / 18, by 8192 x 4096 30 / 18. Eight experts of 1024
-// x 4096 with 128 rows 14 / 18; 64 of 4096 x 2048 with 256 rows 155 / 110:
-// tiles take experts with few rows well if there are enough of them.
-int fewRows(const ProductShape& p, bool grouped, int64_t smallTiles) {
+// better. Measured by 8192 x 4096, this kernel and tiles in us, for bf16
+// results: 1 row 7 / 11, 4 rows 9.4 / 11.1, 16 rows 11.5 / 10.8; for fp32
+// ones, whose tiles take longer: 16 rows 13.7 / 17.1, 32 rows 17.7 / 17.4 (by
+// 4096 x 4096 10 / 17). 32 experts of 4096 x 2048 with 17 rows 28 / 36, with
+// 100 rows among 16 of 1024 x 4096 20 / 14.
+int fewRows(const ProductShape& p, bool grouped, bool exact) {
   if (!p.aWhole || !p.bWhole) {
     return 0;
   }
   if (grouped) {
-    return smallTiles < 256 && p.m <= 16 * p.experts ? 2 : 0;
+    return p.m <= p.experts ? 1 : 0;
   }
-  return p.m <= 16 ? 1 : p.m <= 32 ? 2 : p.m <= 64 && p.n <= 4096 ? 4 : 0;
+  if (exact) {
+    return p.m <= 16 ? 1 : p.m <= 32 ? 2 : 0;
+  }
+  return p.m <= 8 ? 1 : 0;
 }
 
 bool whole16(const void* p, int64_t stride) {
@@ -1322,7 +1333,7 @@ void launchFp8Matmul(
           ((p.n + decltype(tile)::kN - 1) / decltype(tile)::kN);
     };
     const int few = fewRows(
-        p, a.offsets != nullptr, tiles(SmallTile{}));
+        p, a.offsets != nullptr, std::is_same<O, float>::value);
     if (few != 0) {
       const auto goFew = [&](auto rows, auto waves) {
         constexpr int kRows = decltype(rows)::value;
@@ -1342,19 +1353,23 @@ void launchFp8Matmul(
           goFew(rows, std::integral_constant<int, 4>{});
         }
       };
-      if (few == 1) {
-        goWaves(std::integral_constant<int, 1>{});
-      } else if (few == 2) {
-        goWaves(std::integral_constant<int, 2>{});
-      } else {
-        goWaves(std::integral_constant<int, 4>{});
+      if constexpr (std::is_same<O, float>::value) {
+        if (few == 2) {
+          goWaves(std::integral_constant<int, 2>{});
+          return;
+        }
       }
+      goWaves(std::integral_constant<int, 1>{});
       return;
     }
-    if (tiles(LargeTile{}) >= kLargeFrom) {
+    if (tiles(LargeTile{}) >= kEnough) {
       go(matmulKernel<O, 2, 2, 2, 4>, LargeTile{});
-    } else {
+    } else if (tiles(SmallTile{}) >= kEnough) {
       go(matmulKernel<O, 2, 2, 2, 2>, SmallTile{});
+    } else if (tiles(HalfTile{}) >= kEnough) {
+      go(matmulKernel<O, 1, 2, 2, 2>, HalfTile{});
+    } else {
+      go(matmulKernel<O, 1, 1, 2, 2>, QuarterTile{});
     }
   });
   GA_HIP_CHECK(hipGetLastError());
@@ -1393,14 +1408,22 @@ void launchFp8WeightGrad(
           kernel, dim3(gridOf(tiles)), dim3(T::kThreads), 0,
           stream, p, static_cast<O*>(a.out));
     };
-    const int64_t large = (p.m + LargeTile::kM - 1) / LargeTile::kM *
-        ((p.n + LargeTile::kN - 1) / LargeTile::kN) * p.experts;
-    if (large >= kLargeFrom && p.inner / p.experts < kShort * kQuant) {
+    const auto tiles = [&](auto tile) {
+      using T = decltype(tile);
+      return (p.m + T::kM - 1) / T::kM * ((p.n + T::kN - 1) / T::kN) *
+          p.experts;
+    };
+    if (tiles(LargeTile{}) >= kEnough &&
+        p.inner / p.experts < kShort * kQuant) {
       go(weightGradKernel<O, 2, 2, 2, 2, 2>, SmallTile{});
-    } else if (large >= kLargeFrom) {
+    } else if (tiles(LargeTile{}) >= kEnough) {
       go(weightGradKernel<O, 2, 2, 2, 4>, LargeTile{});
-    } else {
+    } else if (tiles(SmallTile{}) >= kEnough) {
       go(weightGradKernel<O, 2, 2, 2, 2>, SmallTile{});
+    } else if (tiles(HalfTile{}) >= kEnough) {
+      go(weightGradKernel<O, 1, 2, 2, 2>, HalfTile{});
+    } else {
+      go(weightGradKernel<O, 1, 1, 2, 2>, QuarterTile{});
     }
   });
   GA_HIP_CHECK(hipGetLastError());
