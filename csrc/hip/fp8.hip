@@ -570,6 +570,10 @@ __device__ inline Float4 multiply(
   return c;
 }
 
+// The widest tiles keep two stages of LDS and a third of half a block in
+// registers (see Product::run).
+constexpr int kWideStages = 4;
+
 // What a workgroup computes: rows [m0, mEnd) by columns from n0 on, over
 // bytes [k0, k1) of the inner dimension.
 struct Job {
@@ -783,32 +787,46 @@ struct Product {
     }
   }
 
+  // The operands of half a block, 64 bytes of the inner dimension.
+  struct Half {
+    Fragment<kExact> a[TM];
+    Fragment<kExact> b[TN];
+  };
+
+  __device__ void
+  read(const uint4* la, const uint4* lb, int h, Half& f) const {
+    const int c = h * 4 + lane / 32 * 2;
+#pragma unroll
+    for (int j = 0; j < TM; j++) {
+      const int r = waveM + j * 32 + lane % 32;
+      f.a[j].set(la[r * kChunks + chunkOf(r, c)],
+                 la[r * kChunks + chunkOf(r, c + 1)], sa[j]);
+    }
+#pragma unroll
+    for (int i = 0; i < TN; i++) {
+      const int r = waveN + i * 32 + lane % 32;
+      f.b[i].set(lb[r * kChunks + chunkOf(r, c)],
+                 lb[r * kChunks + chunkOf(r, c + 1)], sb[i]);
+    }
+  }
+
+  __device__ void add(const Half& f) {
+#pragma unroll
+    for (int i = 0; i < TN; i++) {
+#pragma unroll
+      for (int j = 0; j < TM; j++) {
+        acc[i][j] = multiply(f.b[i], f.a[j], acc[i][j]);
+      }
+    }
+  }
+
   __device__ void step(const uint4* la, const uint4* lb, const int* ls) {
     readScales(ls);
 #pragma unroll
     for (int h = 0; h < 2; h++) {
-      Fragment<kExact> fa[TM];
-      Fragment<kExact> fb[TN];
-      const int c = h * 4 + lane / 32 * 2;
-#pragma unroll
-      for (int j = 0; j < TM; j++) {
-        const int r = waveM + j * 32 + lane % 32;
-        fa[j].set(la[r * kChunks + chunkOf(r, c)],
-                  la[r * kChunks + chunkOf(r, c + 1)], sa[j]);
-      }
-#pragma unroll
-      for (int i = 0; i < TN; i++) {
-        const int r = waveN + i * 32 + lane % 32;
-        fb[i].set(lb[r * kChunks + chunkOf(r, c)],
-                  lb[r * kChunks + chunkOf(r, c + 1)], sb[i]);
-      }
-#pragma unroll
-      for (int i = 0; i < TN; i++) {
-#pragma unroll
-        for (int j = 0; j < TM; j++) {
-          acc[i][j] = multiply(fb[i], fa[j], acc[i][j]);
-        }
-      }
+      Half f;
+      read(la, lb, h, f);
+      add(f);
     }
   }
 
@@ -819,6 +837,7 @@ struct Product {
     constexpr int kSizeA = T::kM * kChunks;
     constexpr int kSizeB = T::kN * kChunks;
     constexpr bool kThree = S == 3;
+    constexpr bool kWide = S == kWideStages;
     __shared__ uint4 la0[kSizeA];
     __shared__ uint4 lb0[kSizeB];
     __shared__ uint4 la1[kSizeA];
@@ -882,7 +901,43 @@ struct Product {
       };
       int t = 0;
       begin(0, la0, lb0, ls0);
-      if constexpr (kThree) {
+      if constexpr (kWide) {
+        // While half a block is multiplied the next half is read. A stage is
+        // free in the middle of its step, and one barrier says both that and
+        // that the next stage has arrived. (Whole blocks alone: the rows of
+        // a product do not part the inner dimension.)
+        begin(1, la1, lb1, ls1);
+        Half f0;
+        Half f1;
+        arrived<StageA::kEach + StageB::kEach + 1>();
+        readScales(ls0);
+        read(la0, lb0, 0, f0);
+        for (; t + 1 < total; t += 2) {
+          read(la0, lb0, 1, f1);
+          add(f0);
+          __builtin_amdgcn_sched_barrier(0);
+          arrived<0>();
+          begin(t + 2, la0, lb0, ls0);
+          readScales(ls1);
+          read(la1, lb1, 0, f0);
+          add(f1);
+          __builtin_amdgcn_sched_barrier(0);
+          read(la1, lb1, 1, f1);
+          add(f0);
+          __builtin_amdgcn_sched_barrier(0);
+          arrived<0>();
+          begin(t + 3, la1, lb1, ls1);
+          readScales(ls0);
+          read(la0, lb0, 0, f0);
+          add(f1);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (t < total) {
+          read(la0, lb0, 1, f1);
+          add(f0);
+          add(f1);
+        }
+      } else if constexpr (kThree) {
         begin(1, la1, lb1, ls1);
         for (; t + 2 < whole; t += 3) {
           arrived<kLater>();
@@ -1162,6 +1217,11 @@ weightGradKernel(ProductShape p, O* __restrict__ out) {
 // weight gradient of 16384 rows, 2048 x 2048 and 1024 x 1024:
 //                          137        97.5     114.9    140.1
 //                                     87.2      58.1     39.6
+// Wider ones still, for 16-bit results: 256 x 256 437, for 32 experts 16384 x
+// 4096 x 4096 332 against 370 us with 128 x 256, if experts have rows for
+// them (64 experts with 256 rows: 131 / 108).
+using WideTile = Tile<2, 4, 4, 2>;
+constexpr int64_t kWideRows = 128;
 using LargeTile = Tile<2, 2, 2, 4>;
 using SmallTile = Tile<2, 2, 2, 2>;
 using HalfTile = Tile<1, 2, 2, 2>;
@@ -1361,6 +1421,12 @@ void launchFp8Matmul(
       }
       goWaves(std::integral_constant<int, 1>{});
       return;
+    }
+    if constexpr (!std::is_same<O, float>::value) {
+      if (tiles(WideTile{}) >= kEnough && p.m >= kWideRows * p.experts) {
+        go(matmulKernel<O, 2, 4, 4, 2, kWideStages>, WideTile{});
+        return;
+      }
     }
     if (tiles(LargeTile{}) >= kEnough) {
       go(matmulKernel<O, 2, 2, 2, 4>, LargeTile{});
