@@ -28,7 +28,20 @@ endif
 HIPCCFLAGS := -O3 -std=c++17 -fPIC -MMD -MP --offload-arch=gfx950 -Icsrc \
   -Xclang -target-feature -Xclang -packed-fp32-ops
 
-CC_SRCS := $(shell find csrc -name '*.cc' ! -path 'csrc/bindings/*' ! -path 'csrc/bench/*')
+# The tensors' side of gloo_amd.experts links torch, and is an extension of its
+# own: gloo_amd._C does without.
+TORCH := $(shell $(PYTHON) -c "import importlib.util as u; \
+  s = u.find_spec('torch'); print(s.submodule_search_locations[0] if s else '')")
+ifneq ($(TORCH),)
+OPERATORS := gloo_amd/_operators$(EXT_SUFFIX)
+endif
+TORCH_FLAGS = -isystem $(TORCH)/include \
+  -isystem $(TORCH)/include/torch/csrc/api/include
+TORCH_LIBS = -L$(TORCH)/lib -Wl,-rpath,$(TORCH)/lib -ltorch_python -ltorch \
+  -ltorch_cpu -lc10
+
+CC_SRCS := $(shell find csrc -name '*.cc' ! -path 'csrc/bindings/*' \
+  ! -path 'csrc/bench/*' ! -path 'csrc/torch/*')
 HIP_SRCS := $(shell find csrc -name '*.hip' 2>/dev/null)
 BIND_SRCS := $(shell find csrc/bindings -name '*.cc')
 
@@ -38,7 +51,7 @@ BIND_OBJS := $(patsubst csrc/%.cc,build/%.o,$(BIND_SRCS))
 
 LDFLAGS := -L$(ROCM)/lib -lamdhip64 -lroctx64 -lssl -lcrypto -luv -pthread $(LDFLAGS_EXTRA)
 
-all: $(TARGET) $(BENCH)
+all: $(TARGET) $(BENCH) $(OPERATORS)
 
 build/%.o: csrc/%.cc
 	@mkdir -p $(dir $@)
@@ -51,8 +64,15 @@ build/%.hip.o: csrc/%.hip
 $(TARGET): $(CC_OBJS) $(HIP_OBJS) $(BIND_OBJS)
 	$(CXX) -shared -o $@ $^ $(LDFLAGS)
 
+build/torch/%.o: csrc/torch/%.cc
+	@mkdir -p $(dir $@)
+	$(CXX) $(CXXFLAGS) $(TORCH_FLAGS) -I$(PY_INC) -c $< -o $@
+
+gloo_amd/_operators$(EXT_SUFFIX): build/torch/operators.o
+	$(CXX) -shared -o $@ $^ $(TORCH_LIBS) $(LDFLAGS_EXTRA)
+
 clean:
-	rm -rf build $(TARGET) $(BENCH)
+	rm -rf build $(TARGET) $(BENCH) $(OPERATORS)
 
 -include $(shell find build -name "*.d" 2>/dev/null)
 

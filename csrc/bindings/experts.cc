@@ -3,6 +3,7 @@
 #include <string>
 
 #include "common/logging.h"
+#include "hip/expert_launchers.h"
 #include "hip/experts.h"
 #include "hip/fp8.h"
 
@@ -55,6 +56,18 @@ void bindExperts(py::module_& m) {
   m.attr("MAX_EXPERTS") = hip::kMaxExperts;
   m.attr("MAX_TOPK") = hip::kMaxTopK;
   m.attr("MAX_EXPERT_GROUPS") = hip::kMaxExpertGroups;
+
+  // For gloo_amd._operators, which does not link the kernels.
+  m.def("expert_launchers", [] {
+    static hip::ExpertLaunchers launchers{
+        &hip::launchRoute, &hip::launchRouteBackward,
+        &hip::expertPlanWorkspace, &hip::launchExpertPlan,
+        &hip::launchExpertPack, &hip::launchExpertPackFp8,
+        &hip::launchExpertCombine, &hip::launchExpertCombineBackward,
+        &hip::launchQuantizeFp8, &hip::launchFp8Matmul,
+        &hip::launchFp8WeightGrad};
+    return py::capsule(&launchers, hip::kExpertLaunchers);
+  });
 
   m.def(
       "hip_expert_route",

@@ -9,9 +9,9 @@
 `pack_fp8` packs in 8 bits with a scale for each block of 128 instead, and
 `fp8_matmul` multiplies such rows by their experts' weights; `ExpertExchange`
 runs the whole way over a process group. All operators are hand-written HIP
-kernels (csrc/hip/experts.hip, csrc/hip/fp8.hip) that run asynchronously on
-the current stream of their tensors' device, allocate with torch's allocator
-and may be captured into a graph. Tensors have to be on a GPU; wrong arguments
+kernels (csrc/hip/experts.hip, csrc/hip/fp8.hip, called by csrc/torch) that
+run asynchronously on the current stream of their tensors' device, allocate
+with torch's allocator and may be captured into a graph. Tensors have to be on a GPU; wrong arguments
 raise ValueError before anything is launched.
 
 8-bit values are torch.float8_e4m3fn. Their scales are powers of two
@@ -25,14 +25,15 @@ import torch
 import torch.distributed as dist
 
 import gloo_amd as ga
+from gloo_amd import _operators as _ops
 
 _C = ga._C
+_ops.set_launchers(_C.expert_launchers())
 
 FP8 = torch.float8_e4m3fn
 FP8_SCALE = torch.float8_e8m0fnu
 FP8_BLOCK = 128
-_FLOATS = {torch.float32: ga.DType.f32, torch.float16: ga.DType.f16,
-           torch.bfloat16: ga.DType.bf16}
+_FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
 class ExpertPlan(NamedTuple):
@@ -88,53 +89,11 @@ def _once():
                            "differentiated again (create_graph=True)")
 
 
-def _adjacent(t):
-    """t, or a copy of it, with adjacent elements in its last dimension."""
-    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
-
-
 def _blocks(n):
     return (n + FP8_BLOCK - 1) // FP8_BLOCK
 
 
 # ------------------------------------------------------------------- router
-
-
-def _route(logits, bias, k, score, groups, topk_groups, group_score,
-           renormalize, scale):
-    x = _adjacent(logits.detach())
-    tokens, experts = x.shape
-    weights = torch.empty(tokens, k, dtype=torch.float32, device=x.device)
-    ids = torch.empty(tokens, k, dtype=torch.int32, device=x.device)
-    _C.hip_expert_route(
-        x.data_ptr(), x.stride(0), _FLOATS[x.dtype],
-        0 if bias is None else bias.data_ptr(), tokens, experts, k, score,
-        groups, topk_groups, group_score, renormalize, scale,
-        weights.data_ptr(), ids.data_ptr(), x.get_device(), _stream(x))
-    return weights, ids
-
-
-class _Route(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, logits, *options):
-        weights, ids = _route(logits, *options)
-        ctx.mark_non_differentiable(ids)
-        ctx.save_for_backward(logits, ids)
-        ctx.options = options
-        return weights, ids
-
-    @staticmethod
-    def backward(ctx, grad, _):
-        _once()
-        logits, ids = ctx.saved_tensors
-        _, k, score, _, _, _, renormalize, scale = ctx.options
-        x, grad = _adjacent(logits.detach()), grad.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        _C.hip_expert_route_backward(
-            x.data_ptr(), x.stride(0), _FLOATS[x.dtype], x.shape[0],
-            x.shape[1], k, score, renormalize, scale, ids.data_ptr(),
-            grad.data_ptr(), dx.data_ptr(), x.get_device(), _stream(x))
-        return dx, None, None, None, None, None, None, None, None
 
 
 def route(logits, k, *, score="softmax", bias=None, groups=1, topk_groups=1,
@@ -191,11 +150,10 @@ def route(logits, k, *, score="softmax", bias=None, groups=1, topk_groups=1,
                 f"bias: {experts} values are needed, got {bias.shape[0]}")
         bias = bias.detach().contiguous()
     _gpu(logits, "route")
-    options = (bias, k, score, groups, topk_groups, group_score,
-               bool(renormalize), float(scale))
-    if _differentiated(logits):
-        return _Route.apply(logits, *options)
-    return _route(logits, *options)
+    return _ops.route(
+        logits, bias, k, score == "sigmoid", groups, topk_groups,
+        group_score == "top2", bool(renormalize), float(scale),
+        _stream(logits))
 
 
 # ------------------------------------------------- plan, pack and combine
@@ -208,27 +166,11 @@ def plan(experts, num_experts):
     if not 1 <= num_experts <= _C.MAX_EXPERTS:
         raise ValueError(
             f"plan: 1 to {_C.MAX_EXPERTS} experts, got {num_experts}")
-    ids = experts.contiguous()
-    n = ids.numel()
-    if n >= 2 ** 31:
-        raise ValueError(f"plan: fewer than 2^31 token copies, got {n}")
-    _gpu(ids, "plan")
-    dev = ids.device
-    position = torch.empty_like(ids)
-    counts = torch.empty(num_experts, dtype=torch.int32, device=dev)
-    offsets = torch.empty(num_experts + 1, dtype=torch.int32, device=dev)
-    size = _C.hip_expert_plan_workspace(n, num_experts)
-    work = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _C.hip_expert_plan(
-        ids.data_ptr(), n, num_experts, position.data_ptr(),
-        counts.data_ptr(), offsets.data_ptr(),
-        work.data_ptr() if size else 0, size, ids.get_device(), _stream(ids))
-    return ExpertPlan(position, counts, offsets)
-
-
-def _rows_args(position, hidden, dtype):
-    return (position.data_ptr(), position.shape[0], position.shape[1],
-            hidden, _FLOATS[dtype])
+    if experts.numel() >= 2 ** 31:
+        raise ValueError(f"plan: fewer than 2^31 token copies, got "
+                         f"{experts.numel()}")
+    _gpu(experts, "plan")
+    return ExpertPlan(*_ops.plan(experts, num_experts, _stream(experts)))
 
 
 def _check_plan(p, tokens, like):
@@ -244,71 +186,6 @@ def _check_plan(p, tokens, like):
     return position
 
 
-def _pack(x, position):
-    x = _adjacent(x)
-    hidden = x.shape[1]
-    rows = torch.empty(position.numel(), hidden, dtype=x.dtype,
-                       device=x.device)
-    if rows.numel():
-        _C.hip_expert_pack(
-            *_rows_args(position, hidden, x.dtype), x.data_ptr(),
-            x.stride(0), rows.data_ptr(), x.get_device(), _stream(x))
-    return rows
-
-
-def _combine(rows, position, weights):
-    rows = _adjacent(rows)
-    hidden = rows.shape[1]
-    out = torch.empty(position.shape[0], hidden, dtype=rows.dtype,
-                      device=rows.device)
-    if out.numel():
-        _C.hip_expert_combine(
-            *_rows_args(position, hidden, rows.dtype), rows.data_ptr(),
-            rows.stride(0), 0 if weights is None else weights.data_ptr(),
-            out.data_ptr(), rows.get_device(), _stream(rows))
-    return out
-
-
-class _Pack(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, position):
-        ctx.save_for_backward(position)
-        return _pack(x.detach(), position)
-
-    @staticmethod
-    def backward(ctx, grad):
-        _once()
-        position, = ctx.saved_tensors
-        return _combine(grad, position, None), None
-
-
-class _Combine(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, rows, position, weights):
-        ctx.save_for_backward(rows, position, weights)
-        return _combine(rows.detach(), position, weights)
-
-    @staticmethod
-    def backward(ctx, grad):
-        _once()
-        rows, position, weights = ctx.saved_tensors
-        if weights is None:
-            return _pack(grad, position), None, None
-        rows, grad = _adjacent(rows.detach()), _adjacent(grad)
-        drows = torch.empty(rows.shape, dtype=rows.dtype, device=rows.device)
-        dw = torch.empty(weights.shape, dtype=torch.float32,
-                         device=rows.device)
-        if drows.numel():
-            _C.hip_expert_combine_backward(
-                *_rows_args(position, rows.shape[1], rows.dtype),
-                rows.data_ptr(), rows.stride(0), weights.data_ptr(),
-                grad.data_ptr(), grad.stride(0), drows.data_ptr(),
-                dw.data_ptr(), rows.get_device(), _stream(rows))
-        else:
-            dw.zero_()
-        return drows, None, dw
-
-
 def pack(x, plan):
     """Copies tokens to their rows: rows[plan.position[t, j]] = x[t].
 
@@ -318,9 +195,7 @@ def pack(x, plan):
     _tensor(x, "x", 2, _FLOATS)
     position = _check_plan(plan, x.shape[0], x)
     _gpu(x, "pack")
-    if _differentiated(x):
-        return _Pack.apply(x, position)
-    return _pack(x.detach(), position)
+    return _ops.pack(x, position, _stream(x))
 
 
 def pack_fp8(x, plan):
@@ -332,17 +207,7 @@ def pack_fp8(x, plan):
     _no_gradient("pack_fp8", x)
     position = _check_plan(plan, x.shape[0], x)
     _gpu(x, "pack_fp8")
-    x = _adjacent(x.detach())
-    hidden, n = x.shape[1], position.numel()
-    q, stride = _fp8_rows((n,), hidden, x.device)
-    scales = torch.empty(n, _blocks(hidden), dtype=FP8_SCALE,
-                         device=x.device)
-    if n and hidden:
-        _C.hip_expert_pack_fp8(
-            *_rows_args(position, hidden, x.dtype), x.data_ptr(),
-            x.stride(0), q.data_ptr(), stride, scales.data_ptr(),
-            x.get_device(), _stream(x))
-    return q, scales
+    return _ops.pack_fp8(x, position, _stream(x))
 
 
 def combine(rows, plan, weights=None):
@@ -364,11 +229,9 @@ def combine(rows, plan, weights=None):
             raise ValueError(
                 f"weights: {tuple(position.shape)} is needed, got "
                 f"{tuple(weights.shape)}")
-        weights = weights.contiguous()
+        weights = weights.contiguous()  # a part of the gradient's way
     _gpu(rows, "combine")
-    if _differentiated(rows, weights):
-        return _Combine.apply(rows, position, weights)
-    return _combine(rows.detach(), position, weights)
+    return _ops.combine(rows, position, weights, _stream(rows))
 
 
 # ------------------------------------------------------------ 8-bit products
@@ -377,16 +240,6 @@ def combine(rows, plan, weights=None):
 def _no_gradient(name, *tensors):
     if _differentiated(*tensors):
         raise ValueError(f"{name} has no gradient: detach() its inputs")
-
-
-def _fp8_rows(shape, width, device):
-    """Room for rows of `width` 8-bit values that begin on borders of 128
-    bytes, so that products can load them whole."""
-    stride = _blocks(width) * FP8_BLOCK
-    if stride == width:
-        return torch.empty(*shape, width, dtype=FP8, device=device), stride
-    q = torch.empty(*shape, stride, dtype=torch.uint8, device=device)
-    return q.view(FP8)[..., :width], stride
 
 
 def quantize_fp8(x, tile=False):
@@ -399,39 +252,14 @@ def quantize_fp8(x, tile=False):
     ceil(cols / 128)], and x may have a leading dimension for experts. For
     scales along the columns (a weight gradient's operands) quantise x.t().
     Rows of q begin on borders of 128 bytes. It has no gradient."""
-    if tile and isinstance(x, torch.Tensor) and x.dim() == 3:
-        _tensor(x, "x", 3, _FLOATS)
-        _no_gradient("quantize_fp8", x)
-        _gpu(x, "quantize_fp8")
-        experts, rows, cols = x.shape
-        q, stride = _fp8_rows((experts, rows), cols, x.device)
-        scales = torch.empty(experts, _blocks(rows), _blocks(cols),
-                             dtype=FP8_SCALE, device=x.device)
-        for e in range(experts):
-            _quantize(x[e], True, q[e], stride, scales[e])
-        return q, scales
-    _tensor(x, "x", 2, _FLOATS)
+    three = tile and isinstance(x, torch.Tensor) and x.dim() == 3
+    _tensor(x, "x", 3 if three else 2, _FLOATS)
     _no_gradient("quantize_fp8", x)
+    if x.shape[-1] > 65535 * FP8_BLOCK:
+        raise ValueError(f"quantize_fp8: at most {65535 * FP8_BLOCK} "
+                         f"columns, got {x.shape[-1]}")
     _gpu(x, "quantize_fp8")
-    rows, cols = x.shape
-    q, stride = _fp8_rows((rows,), cols, x.device)
-    scales = torch.empty(_blocks(rows) if tile else rows, _blocks(cols),
-                         dtype=FP8_SCALE, device=x.device)
-    _quantize(x, bool(tile), q, stride, scales)
-    return q, scales
-
-
-def _quantize(x, tile, q, stride, scales):
-    x = x.detach()
-    if x.shape[1] > 65535 * FP8_BLOCK:
-        raise ValueError(
-            f"quantize_fp8: at most {65535 * FP8_BLOCK} columns, got "
-            f"{x.shape[1]}")
-    if x.numel():
-        _C.hip_quantize_fp8(
-            x.data_ptr(), x.stride(0), x.stride(1), _FLOATS[x.dtype],
-            x.shape[0], x.shape[1], tile, q.data_ptr(), stride,
-            scales.data_ptr(), x.get_device(), _stream(x))
+    return _ops.quantize_fp8(x, bool(tile), _stream(x))
 
 
 def _fp8_operand(q, scale, name, dim, scale_shape, like=None):
@@ -440,24 +268,15 @@ def _fp8_operand(q, scale, name, dim, scale_shape, like=None):
     if tuple(scale.shape) != scale_shape:
         raise ValueError(f"{name}_scale: {scale_shape} is needed, got "
                          f"{tuple(scale.shape)}")
-    return _adjacent(q), scale.contiguous()
-
-
-def _pitch(q):
-    """Bytes from one row to the next; a single row has none, whatever its
-    stride says, and begins where the tensor does."""
-    return q.stride(-2) if q.shape[-2] > 1 else 0
 
 
 def _offsets(offsets, experts, like):
     if offsets is None:
-        return 0
+        return
     _tensor(offsets, "offsets", 1, (torch.int32,), like)
     if offsets.shape[0] != experts + 1 or not offsets.is_contiguous():
-        raise ValueError(
-            f"offsets: {experts + 1} adjacent numbers are needed, got "
-            f"{tuple(offsets.shape)}")
-    return offsets.data_ptr()
+        raise ValueError(f"offsets: {experts + 1} adjacent numbers are "
+                         f"needed, got {tuple(offsets.shape)}")
 
 
 def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
@@ -487,20 +306,13 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
             f"b: an inner dimension of {inner} is needed, got {b.shape[-1]}")
     if n <= 0 or experts <= 0:
         raise ValueError(f"b: got {tuple(b.shape)}")
-    a, a_scale = _fp8_operand(a, a_scale, "a", 2, (rows, _blocks(inner)))
-    b, b_scale = _fp8_operand(
-        b, b_scale, "b", b.dim(),
-        tuple(b.shape[:-2]) + (_blocks(n), _blocks(inner)), a)
-    at = _offsets(offsets, experts, a)
+    _fp8_operand(a, a_scale, "a", 2, (rows, _blocks(inner)))
+    _fp8_operand(b, b_scale, "b", b.dim(),
+                 tuple(b.shape[:-2]) + (_blocks(n), _blocks(inner)), a)
+    _offsets(offsets, experts, a)
     _gpu(a, "fp8_matmul")
-    out = torch.empty(rows, n, dtype=dtype, device=a.device)
-    if rows:
-        _C.hip_fp8_matmul(
-            a.data_ptr(), _pitch(a), a_scale.data_ptr(), b.data_ptr(),
-            _pitch(b), 0 if offsets is None else b.stride(0),
-            b_scale.data_ptr(), at, rows, n, inner, experts, out.data_ptr(),
-            _FLOATS[dtype], a.get_device(), _stream(a))
-    return out
+    return _ops.fp8_matmul(a, a_scale, b, b_scale, offsets, dtype,
+                           _stream(a))
 
 
 def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
@@ -525,23 +337,16 @@ def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
     if m <= 0 or n <= 0:
         raise ValueError(f"dy, x: got {tuple(dy.shape)}, "
                          f"{tuple(x.shape)}")
-    dy, dy_scale = _fp8_operand(dy, dy_scale, "dy", 2, (m, _blocks(rows)))
-    x, x_scale = _fp8_operand(x, x_scale, "x", 2, (n, _blocks(rows)), dy)
-    experts = 1
-    if offsets is not None:
-        if (not isinstance(offsets, torch.Tensor) or offsets.dim() != 1
-                or offsets.shape[0] <= 1):
-            raise ValueError("offsets: [experts + 1] is needed")
-        experts = offsets.shape[0] - 1
-    at = _offsets(offsets, experts, dy)
+    _fp8_operand(dy, dy_scale, "dy", 2, (m, _blocks(rows)))
+    _fp8_operand(x, x_scale, "x", 2, (n, _blocks(rows)), dy)
+    if offsets is not None and (
+            not isinstance(offsets, torch.Tensor) or offsets.dim() != 1
+            or offsets.shape[0] < 2):
+        raise ValueError("offsets: [experts + 1] is needed")
+    _offsets(offsets, 0 if offsets is None else offsets.shape[0] - 1, dy)
     _gpu(dy, "fp8_weight_grad")
-    out = torch.empty((m, n) if offsets is None else (experts, m, n),
-                      dtype=dtype, device=dy.device)
-    _C.hip_fp8_weight_grad(
-        dy.data_ptr(), _pitch(dy), dy_scale.data_ptr(), x.data_ptr(),
-        _pitch(x), x_scale.data_ptr(), at, m, n, rows, experts,
-        out.data_ptr(), _FLOATS[dtype], dy.get_device(), _stream(dy))
-    return out
+    return _ops.fp8_weight_grad(dy, dy_scale, x, x_scale, offsets, dtype,
+                                _stream(dy))
 
 
 # ------------------------------------------------------- over a process group

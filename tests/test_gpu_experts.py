@@ -954,6 +954,71 @@ def test_training_step_captured():
             assert torch.equal(a, b)
 
 
+def test_raw_entry_points():
+    """The same kernels by device pointers, on the null stream."""
+    gen = torch.Generator().manual_seed(15)
+    c, f = ga._C, ga.DType.f32
+    t, k, e, h = 50, 3, 7, 256
+    x = torch.randn(t, e, generator=gen).cuda()
+    w = torch.empty(t, k, device="cuda")
+    ids = torch.empty(t, k, dtype=torch.int32, device="cuda")
+    c.hip_expert_route(x.data_ptr(), e, f, 0, t, e, k, "sigmoid", 1, 1, "max",
+                       True, 1.0, w.data_ptr(), ids.data_ptr(), 0, 0)
+    rw, rid = ex.route(x, k, score="sigmoid")
+    assert torch.equal(ids, rid) and torch.equal(w, rw)
+    g, dx = torch.ones_like(w), torch.empty_like(x)
+    c.hip_expert_route_backward(
+        x.data_ptr(), e, f, t, e, k, "sigmoid", False, 1.0, ids.data_ptr(),
+        g.data_ptr(), dx.data_ptr(), 0, 0)
+    y = x.clone().requires_grad_()
+    ex.route(y, k, score="sigmoid", renormalize=False)[0].sum().backward()
+    assert torch.equal(dx, y.grad)
+    p = ex.plan(ids, e)
+    pos, cnt, off = (torch.empty_like(v) for v in p)
+    size = c.hip_expert_plan_workspace(t * k, e)
+    work = torch.empty(max(size, 1), dtype=torch.uint8, device="cuda")
+    c.hip_expert_plan(ids.data_ptr(), t * k, e, pos.data_ptr(),
+                      cnt.data_ptr(), off.data_ptr(), work.data_ptr(), size,
+                      0, 0)
+    assert all(torch.equal(a, b) for a, b in zip(p, (pos, cnt, off)))
+    v = torch.randn(t, h, generator=gen).cuda()
+    rows = torch.empty(t * k, h, device="cuda")
+    c.hip_expert_pack(pos.data_ptr(), t, k, h, f, v.data_ptr(), h,
+                      rows.data_ptr(), 0, 0)
+    assert torch.equal(rows, ex.pack(v, p))
+    out, drows, dw = (torch.empty_like(i) for i in (v, rows, w))
+    c.hip_expert_combine(pos.data_ptr(), t, k, h, f, rows.data_ptr(), h,
+                         w.data_ptr(), out.data_ptr(), 0, 0)
+    r, q = rows.clone().requires_grad_(), w.clone().requires_grad_()
+    ref = ex.combine(r, p, q)
+    assert torch.equal(out, ref)
+    c.hip_expert_combine_backward(
+        pos.data_ptr(), t, k, h, f, rows.data_ptr(), h, w.data_ptr(),
+        v.data_ptr(), h, drows.data_ptr(), dw.data_ptr(), 0, 0)
+    ref.backward(v)
+    assert torch.equal(drows, r.grad) and torch.equal(dw, q.grad)
+    a = torch.empty(t * k, h, dtype=F8, device="cuda")
+    s = torch.empty(t * k, 2, dtype=E8, device="cuda")
+    c.hip_expert_pack_fp8(pos.data_ptr(), t, k, h, f, v.data_ptr(), h,
+                          a.data_ptr(), h, s.data_ptr(), 0, 0)
+    a2, s2 = torch.empty_like(a), torch.empty_like(s)
+    c.hip_quantize_fp8(rows.data_ptr(), h, 1, f, t * k, h, False,
+                       a2.data_ptr(), h, s2.data_ptr(), 0, 0)
+    assert torch.equal(a.float(), a2.float())
+    assert torch.equal(s.float(), s2.float())
+    b, bs = ex.quantize_fp8(torch.randn(64, h, generator=gen).cuda(), True)
+    y = torch.empty(t * k, 64, device="cuda")
+    c.hip_fp8_matmul(a.data_ptr(), h, s.data_ptr(), b.data_ptr(), h, 0,
+                     bs.data_ptr(), 0, t * k, 64, h, 1, y.data_ptr(), f, 0,
+                     0)
+    assert torch.equal(y, ex.fp8_matmul(a, s, b, bs, dtype=torch.float32))
+    y = torch.empty(t * k, t * k, device="cuda")
+    c.hip_fp8_weight_grad(a.data_ptr(), h, s.data_ptr(), a.data_ptr(), h,
+                          s.data_ptr(), 0, t * k, t * k, h, 1, y.data_ptr(),
+                          f, 0, 0)
+    assert torch.equal(y, ex.fp8_weight_grad(a, s, a, s))
+
+
 def test_same_results_every_time():
     gen = torch.Generator().manual_seed(14)
     t, k, e, h = 3000, 8, 64, 256
