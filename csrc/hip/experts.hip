@@ -324,43 +324,48 @@ __global__ __launch_bounds__(kBlock) void routeKernel(
     if (best == 0) {
       break; // none is left
     }
-    // the first of this lane's that has it, and how many have
-    int at = 0;
+    // Who has it, as masks: what follows from them is the scalar unit's work.
+    uint64_t have[kPer];
+    uint64_t any = 0;
     int count = 0;
-    float l = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; i++) {
+      have[i] = __ballot(order[i] == best);
+      any |= have[i];
+      count += kBias ? __popcll(have[i]) : 0;
+    }
+    int winner = __ffsll(static_cast<unsigned long long>(any)) - 1;
+    int at = 0;
 #pragma unroll
     for (int i = kPer - 1; i >= 0; i--) {
-      const bool is = order[i] == best;
-      at = is ? i : at;
-      l = is ? logit[i] : l;
-      count += kBias && is;
+      at = have[i] >> winner & 1 ? i : at;
     }
-    const uint64_t have = __ballot(most == best);
-    int winner = __ffsll(static_cast<unsigned long long>(have)) - 1;
-    if (kBias &&
-        (have & (have - 1) || __builtin_amdgcn_readlane(count, winner) > 1)) {
+    if (kBias && count > 1) {
       double r = none;
+      int own = 0;
 #pragma unroll
       for (int i = kPer - 1; i >= 0; i--) {
         const bool is = order[i] == best && rank[i] >= r;
-        at = is ? i : at;
-        l = is ? logit[i] : l;
+        own = is ? i : own;
         r = is ? rank[i] : r;
       }
       double highest = none;
-      for (uint64_t rest = have; rest != 0; rest &= rest - 1) {
+      for (uint64_t rest = any; rest != 0; rest &= rest - 1) {
         const int of = __ffsll(static_cast<unsigned long long>(rest)) - 1;
         const double other = laneOf(r, of);
         winner = other > highest ? of : winner;
         highest = other > highest ? other : highest;
       }
+      at = __builtin_amdgcn_readlane(own, winner);
     }
-    const int expert =
-        winner * kPer + __builtin_amdgcn_readlane(at, winner);
-    const float value = laneOf(l, winner);
+    const int expert = winner * kPer + at;
+    float value = 0;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
-      order[i] = first + i == expert ? 0 : order[i];
+      if (at == i) { // the same in every lane
+        value = laneOf(logit[i], winner);
+        order[i] = lane == winner ? 0 : order[i];
+      }
     }
     if (lane == j) {
       mine = expert;
