@@ -61,6 +61,12 @@ __device__ inline __hip_bfloat16 fromFloat<__hip_bfloat16>(float v) {
   return __float2bfloat16(v);
 }
 
+// Workgroups along x: a launch has fewer than 2^32 threads there.
+inline unsigned groupsOf(int64_t groups, int threads) {
+  GA_ENFORCE_LE(groups, UINT32_MAX / threads);
+  return static_cast<unsigned>(groups);
+}
+
 // 16 bytes of T, moved as one load or store.
 template <typename T>
 struct alignas(16) Vec16 {

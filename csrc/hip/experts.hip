@@ -566,7 +566,6 @@ RouteShape checkRoute(const RouteArgs& a) {
   GA_ENFORCE_GT(a.topkGroups, 0);
   GA_ENFORCE_LE(a.topkGroups, a.groups);
   GA_ENFORCE_GE(a.stride, 0);
-  GA_ENFORCE_LE((a.tokens + kWaves - 1) / kWaves, INT32_MAX);
   return RouteShape{a.stride,    a.tokens,     a.experts, a.k,
                     a.groups,    a.topkGroups, a.sigmoid, a.groupTop2,
                     a.renormalize, a.scale, false};
@@ -787,7 +786,7 @@ __device__ inline int64_t rowOf(int32_t position, int64_t rows) {
   return row < rows ? row : -1;
 }
 
-// 1, 2, 4 or 16 bytes as one register value, so that masking it takes no
+// 2, 4 or 16 bytes as one register value, so that masking it takes no
 // memory.
 template <int kBytes>
 struct RawOf;
@@ -1080,7 +1079,7 @@ bool wholeVectors(int64_t hidden, int64_t stride, int64_t stride2) {
 dim3 rowsGrid(const RowsShape& p, int64_t width, int each) {
   const int64_t span = static_cast<int64_t>(kBlock) * each;
   return dim3(
-      static_cast<unsigned>(p.tokens),
+      groupsOf(p.tokens, kBlock),
       static_cast<unsigned>((width + span - 1) / span));
 }
 
@@ -1092,7 +1091,7 @@ void launchRoute(const RouteArgs& a, int device, hipStream_t stream) {
     return;
   }
   DeviceGuard guard(device);
-  const dim3 grid(static_cast<unsigned>((p.tokens + kWaves - 1) / kWaves));
+  const dim3 grid(groupsOf((p.tokens + kWaves - 1) / kWaves, kBlock));
   const size_t lds =
       p.groups > 1 ? sizeof(double) * kWaves * p.experts : 0;
   dispatchFloat(a.dtype, "route", [&](auto t) {
@@ -1126,7 +1125,7 @@ void launchRouteBackward(
     return;
   }
   DeviceGuard guard(device);
-  const dim3 grid(static_cast<unsigned>((p.tokens + kWaves - 1) / kWaves));
+  const dim3 grid(groupsOf((p.tokens + kWaves - 1) / kWaves, kBlock));
   dispatchFloat(a.dtype, "route", [&](auto t) {
     using T = decltype(t);
     withPerLane(p.experts, [&](auto per) {
@@ -1317,7 +1316,7 @@ void launchExpertCombineBackward(
       constexpr int kVec = decltype(vec)::value;
       hipLaunchKernelGGL(
           (combineBackwardKernel<T, kVec, 8>),
-          dim3(static_cast<unsigned>(p.tokens)), dim3(kBlock), 0, stream,
+          dim3(groupsOf(p.tokens, kBlock)), dim3(kBlock), 0, stream,
           static_cast<const T*>(rows), rowStride, a.position, weights,
           static_cast<const T*>(grad), gradStride, static_cast<T*>(drows),
           dweights, p);

@@ -388,10 +388,8 @@ __device__ inline bool tileAt(int tilesM, int tilesN, TileAt& at) {
   return true;
 }
 
-unsigned gridOf(int64_t tiles) {
-  tiles = (tiles + kDies - 1) / kDies * kDies;
-  GA_ENFORCE_LE(tiles, INT32_MAX);
-  return static_cast<unsigned>(tiles);
+unsigned gridOf(int64_t tiles, int threads) {
+  return groupsOf((tiles + kDies - 1) / kDies * kDies, threads);
 }
 
 // One operand of a product: rows of bytes, `rows` of them from `p` on.
@@ -831,8 +829,8 @@ struct Product {
   }
 
   // A ring of three stages of LDS, two on their way while one is multiplied,
-  // or of two, one on its way. Arrays of their own and not parts of one: the compiler sees
-  // that a read of one does not wait for loads into another.
+  // or of two, one on its way. Arrays of their own and not parts of one: the
+  // compiler sees that a read of one does not wait for loads into another.
   __device__ void run() {
     constexpr int kSizeA = T::kM * kChunks;
     constexpr int kSizeB = T::kN * kChunks;
@@ -1229,9 +1227,9 @@ using QuarterTile = Tile<1, 1, 2, 2>;
 constexpr int64_t kEnough = 192;
 // A weight gradient of experts with few rows is done with a tile after a few
 // steps: two workgroups with small tiles on a compute unit, with two stages of
-// LDS each, store and multiply at the same time. 16 experts, 16384 x 4096 x 2048 (about eight
-// steps): 388 us against 448 with the large tile for fp32 results, 288 / 351
-// for bf16; from some 30 steps on the large tile is ahead.
+// LDS each, store and multiply at the same time. 16 experts, 16384 x 4096 x
+// 2048 (about eight steps): 388 us against 448 with the large tile for fp32
+// results, 288 / 351 for bf16; from some 30 steps on the large tile is ahead.
 constexpr int kShort = 32;
 
 // Tiles of rows, at most: every expert's last one may be a part of one, and
@@ -1322,8 +1320,7 @@ void launchQuantizeFp8(
     } else if (colStride == 1) {
       const int64_t lanes =
           rows * ((qStride + kQuant - 1) / kQuant * 8);
-      GA_ENFORCE_LE((lanes + 255) / 256, INT32_MAX);
-      const dim3 grid(static_cast<unsigned>((lanes + 255) / 256));
+      const dim3 grid(groupsOf((lanes + 255) / 256, 256));
       if (aligned16(x) && rowStride % Vec16<T>::kSize == 0) {
         hipLaunchKernelGGL(
             (quantizeRowsKernel<T, true>), grid, dim3(256), 0, stream, from,
@@ -1385,7 +1382,7 @@ void launchFp8Matmul(
       p.tilesN = static_cast<int>((p.n + T::kN - 1) / T::kN);
       const int64_t tilesM = tilesOf(tile, p, a.offsets != nullptr);
       hipLaunchKernelGGL(
-          kernel, dim3(gridOf(tilesM * p.tilesN)),
+          kernel, dim3(gridOf(tilesM * p.tilesN, T::kThreads)),
           dim3(T::kThreads), 0, stream, p, static_cast<O*>(a.out));
     };
     const auto tiles = [&](auto tile) {
@@ -1399,7 +1396,7 @@ void launchFp8Matmul(
         constexpr int kRows = decltype(rows)::value;
         constexpr int kWaves = decltype(waves)::value;
         const dim3 grid(
-            static_cast<unsigned>((p.n + 15) / 16),
+            groupsOf((p.n + 15) / 16, kWaves * kWave),
             a.offsets != nullptr ? p.experts + 1 : 1);
         hipLaunchKernelGGL(
             (fewRowsKernel<O, kRows, kWaves>), grid, dim3(kWaves * kWave), 0,
@@ -1471,7 +1468,7 @@ void launchFp8WeightGrad(
       const int64_t tiles =
           (p.m + T::kM - 1) / T::kM * p.tilesN * p.experts;
       hipLaunchKernelGGL(
-          kernel, dim3(gridOf(tiles)), dim3(T::kThreads), 0,
+          kernel, dim3(gridOf(tiles, T::kThreads)), dim3(T::kThreads), 0,
           stream, p, static_cast<O*>(a.out));
     };
     const auto tiles = [&](auto tile) {

@@ -123,6 +123,8 @@ def route(logits, k, *, score="softmax", bias=None, groups=1, topk_groups=1,
     if not 1 <= experts <= _C.MAX_EXPERTS:
         raise ValueError(
             f"route: 1 to {_C.MAX_EXPERTS} experts, got {experts}")
+    if tokens >= 2 ** 26 - 4:
+        raise ValueError(f"route: fewer than 2^26 - 4 tokens, got {tokens}")
     if not 1 <= k <= min(experts, _C.MAX_TOPK):
         raise ValueError(
             f"route: k is 1 to {min(experts, _C.MAX_TOPK)} here, got {k}")
@@ -181,8 +183,13 @@ def _check_plan(p, tokens, like):
     if tokens is not None and position.shape[0] != tokens:
         raise ValueError(
             f"the plan is for {position.shape[0]} tokens, got {tokens}")
-    if position.shape[1] <= 0 or position.numel() >= 2 ** 31:
-        raise ValueError(f"plan.position: got {tuple(position.shape)}")
+    if (position.shape[1] <= 0 or position.numel() >= 2 ** 31
+            or position.shape[0] >= 2 ** 24):
+        raise ValueError(f"plan.position: at least one copy of a token, and "
+                         f"fewer than 2^24 tokens and 2^31 copies, got "
+                         f"{tuple(position.shape)}")
+    if like.shape[1] > 2 ** 23:
+        raise ValueError(f"rows: at most 2^23 elements, got {like.shape[1]}")
     return position
 
 
@@ -258,6 +265,9 @@ def quantize_fp8(x, tile=False):
     if x.shape[-1] > 65535 * FP8_BLOCK:
         raise ValueError(f"quantize_fp8: at most {65535 * FP8_BLOCK} "
                          f"columns, got {x.shape[-1]}")
+    if x.shape[-2] * _blocks(x.shape[-1]) >= 2 ** 29 - 32:
+        raise ValueError(f"quantize_fp8: fewer than 2^29 - 32 blocks, got "
+                         f"{tuple(x.shape)}")
     _gpu(x, "quantize_fp8")
     return _ops.quantize_fp8(x, bool(tile), _stream(x))
 

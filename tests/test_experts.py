@@ -93,6 +93,27 @@ def test_rows_refuse():
                    torch.zeros(4, 2, dtype=torch.bfloat16))
 
 
+def test_what_is_too_large_is_refused():
+    # one element's memory each
+    one = torch.zeros(1)
+    with pytest.raises(ValueError, match="tokens"):
+        ex.route(one.expand(2 ** 26, 8), 2)
+    with pytest.raises(ValueError, match="copies"):
+        ex.plan(torch.zeros(1, dtype=torch.int32).expand(2 ** 30, 2), 8)
+    with pytest.raises(ValueError, match="blocks"):
+        ex.quantize_fp8(one.expand(2 ** 28, 256))
+    with pytest.raises(ValueError, match="columns"):
+        ex.quantize_fp8(one.expand(1, 2 ** 23))
+    p = ex.ExpertPlan(torch.empty(2 ** 24, 1, dtype=torch.int32), None, None)
+    for call in (lambda: ex.pack(one.expand(2 ** 24, 8), p),
+                 lambda: ex.pack_fp8(one.expand(2 ** 24, 8), p),
+                 lambda: ex.combine(one.expand(2 ** 24, 8), p)):
+        with pytest.raises(ValueError, match="fewer than 2"):
+            call()
+    with pytest.raises(ValueError, match="elements"):
+        ex.pack(one.expand(4, 2 ** 23 + 1), _plan())
+
+
 def _operands(rows=4, n=8, inner=200, experts=0):
     b = (experts, n, inner) if experts else (n, inner)
     bs = ((experts,) if experts else ()) + (-(-n // 128), -(-inner // 128))
