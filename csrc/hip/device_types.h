@@ -67,6 +67,11 @@ inline unsigned groupsOf(int64_t groups, int threads) {
   return static_cast<unsigned>(groups);
 }
 
+// Stores past the caches where what a kernel writes would not stay in them
+// anyhow: half of the 256 MB behind the dies' own ones. Below that the next
+// kernel finds it there.
+constexpr int64_t kStreamFrom = 128 << 20;
+
 // 16 bytes of T, moved as one load or store.
 template <typename T>
 struct alignas(16) Vec16 {

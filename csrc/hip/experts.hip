@@ -803,11 +803,6 @@ struct RawOf<16> {
   using type = uint32_t __attribute__((ext_vector_type(4)));
 };
 
-// Stores past the caches where what a kernel writes would not stay in them
-// anyhow: half of the 256 MB behind the dies' own ones. Below that the next
-// kernel finds it there.
-constexpr int64_t kStreamFrom = 128 << 20;
-
 template <bool kStream, typename V>
 __device__ inline void store(V* to, V v) {
   if (kStream) {
