@@ -1372,17 +1372,17 @@ weightGradKernel(ProductShape p, O* __restrict__ out) {
 // them: the largest is taken of which there are enough, most of the 256
 // compute units having one. Measured for bf16 results, in us:
 //                       128 x 256  128 x 128  64 x 128  64 x 64
-//   8192 x 8192 x 8192     454       560
-//   1024 x 4096 x 4096                23.5      24.7     30.3
-//    512 x 4096 x 4096      27        19.7      15.0     16.0
-//    256 x 4096 x 4096                18.9      12.3      9.8
-//   1024 x 2048 x 2048      17        13.1      10.2     11.0
+//   8192 x 8192 x 8192     478       590        652      864
+//   1024 x 4096 x 4096      28.7      22.0      24.8     30.6
+//    512 x 4096 x 4096      26.5      19.3      14.6     16.7
+//    256 x 4096 x 4096      25.4      18.2      11.9      9.8
+//   1024 x 2048 x 2048      16.1      12.1       9.0      9.8
 // weight gradient of 16384 rows, 2048 x 2048 and 1024 x 1024:
-//                          137        97.5     114.9    140.1
-//                                     87.2      58.1     39.6
-// Wider ones still, for 16-bit results: 256 x 256 437, for 32 experts 16384 x
-// 4096 x 4096 332 against 370 us with 128 x 256, if experts have rows for
-// them (64 experts with 256 rows: 131 / 108).
+//                          139        92.8     108.9    136.1
+//                          136        86.9      57.1     39.2
+// Wider ones still, for 16-bit results: 256 x 256 424 for the first of these,
+// for 32 experts 16384 x 4096 x 4096 318 against 356 us with 128 x 256, if
+// experts have rows for them (each has a part of a tile that is empty).
 using WideTile = Tile<2, 4, 4, 2>;
 constexpr int64_t kWideRows = 128;
 using LargeTile = Tile<2, 2, 2, 4>;
@@ -1393,8 +1393,9 @@ constexpr int64_t kEnough = 192;
 // A weight gradient of experts with few rows is done with a tile after a few
 // steps: two workgroups with small tiles on a compute unit, with two stages of
 // LDS each, store and multiply at the same time. 16 experts, 16384 x 4096 x
-// 2048 (about eight steps): 388 us against 448 with the large tile for fp32
-// results, 288 / 351 for bf16; from some 30 steps on the large tile is ahead.
+// 2048 (about eight steps): 391 us against 445 with the large tile for fp32
+// results, 270 / 302 for bf16; 4 experts 355 / 350 and 242 / 246, one expert
+// behind.
 constexpr int kShort = 32;
 
 // Tiles of rows, at most: every expert's last one may be a part of one, and
@@ -1407,16 +1408,17 @@ int64_t tilesOf(T, const ProductShape& p, bool grouped) {
 
 // How many times 16 rows fewRowsKernel takes at a time, 0 where tiles are
 // better. Measured by 8192 x 4096, this kernel and tiles in us, for bf16
-// results: 1 row 7 / 11, 4 rows 9.4 / 11.1, 16 rows 11.5 / 10.8; for fp32
-// ones, whose tiles take longer: 16 rows 13.7 / 17.1, 32 rows 17.7 / 17.4 (by
-// 4096 x 4096 10 / 17). 32 experts of 4096 x 2048 with 17 rows 28 / 36, with
-// 100 rows among 16 of 1024 x 4096 20 / 14.
+// results: 1 row 7 / 10.4, 4 rows 8.2 / 10.2, 16 rows 10.8 / 10.6; for fp32
+// ones, whose tiles take longer: 16 rows 13.6 / 15.2, 32 rows 18.1 / 15.4 (by
+// 4096 x 4096 10.4 / 15.5). 8 rows for 8 of 16 experts of 1024 x 4096 8.5 /
+// 11.9, of 32 of 4096 x 2048 14.9 / 13.8, 16 rows of 16 experts 19.6 / 13.4;
+// fp32 4 rows 8.2 / 16.5 and 11.3 / 10.9, 8 rows 12.6 / 16.5 and 18.8 / 15.7.
 int fewRows(const ProductShape& p, bool grouped, bool exact) {
   if (!p.aWhole || !p.bWhole) {
     return 0;
   }
   if (grouped) {
-    return p.m <= p.experts ? 1 : 0;
+    return p.m <= (exact ? 4 : 8) ? 1 : 0;
   }
   if (exact) {
     return p.m <= 16 ? 1 : p.m <= 32 ? 2 : 0;

@@ -771,6 +771,37 @@ def test_weight_grad_of_neighbours_with_nan():
                   (x.double() * wide_scale(sx, 700, 1))[:, i:j])
 
 
+@pytest.mark.parametrize("out", DTYPES)
+@pytest.mark.parametrize("n", [4200, 4202, 4207])
+def test_results_larger_than_the_caches(n, out):
+    """Whole numbers, whose sums are exact: results that fill 16 bytes, 8 and
+    none, of tiles that are not full, past the size from which they are
+    stored past the caches."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+
+    def whole(*shape):
+        return torch.randint(-3, 4, shape, generator=gen,
+                             device="cuda").float()
+
+    def one(*shape):
+        return torch.ones(shape, device="cuda").to(E8)
+
+    m, k = 17001, 72
+    a, b = whole(m, k), whole(n, k)
+    got = ex.fp8_matmul(a.to(F8), one(m, 1), b.to(F8), one(nb(n), 1),
+                        dtype=out)
+    assert torch.equal(got, (a @ b.t()).to(out))
+    e, m, k = 5, 3501, 300
+    a, b = whole(m, k), whole(n, k)
+    at = [0, 70, 70, 71, 290, k - 3]
+    got = ex.fp8_weight_grad(
+        a.to(F8), one(m, nb(k)), b.to(F8), one(n, nb(k)), dtype=out,
+        offsets=torch.tensor(at, dtype=torch.int32).cuda())
+    for i in range(e):
+        part = slice(at[i], at[i + 1])
+        assert torch.equal(got[i], (a[:, part] @ b[:, part].t()).to(out))
+
+
 def test_single_rows_of_any_stride():
     gen = torch.Generator().manual_seed(6)
     a, sa = operand((1, 512), (1, 4), gen)
