@@ -64,8 +64,8 @@ void bindExperts(py::module_& m) {
         &hip::expertPlanWorkspace, &hip::launchExpertPlan,
         &hip::launchExpertPack, &hip::launchExpertPackFp8,
         &hip::launchExpertCombine, &hip::launchExpertCombineBackward,
-        &hip::launchQuantizeFp8, &hip::launchFp8Matmul,
-        &hip::launchFp8WeightGrad};
+        &hip::launchQuantizeFp8, &hip::launchQuantizeFp8Tiles,
+        &hip::launchFp8Matmul, &hip::launchFp8WeightGrad};
     return py::capsule(&launchers, hip::kExpertLaunchers);
   });
 
@@ -188,10 +188,17 @@ void bindExperts(py::module_& m) {
          int64_t rows, int64_t cols, bool tile, uintptr_t q, int64_t qStride,
          uintptr_t scales, int device, uintptr_t stream) {
         py::gil_scoped_release rel;
-        hip::launchQuantizeFp8(
-            ptr<const void>(x), rowStride, colStride, dtype, rows, cols,
-            tile, ptr<void>(q), qStride, ptr<void>(scales), device,
-            toStream(stream));
+        if (tile) {
+          hip::launchQuantizeFp8Tiles(
+              ptr<const void>(x), 0, rowStride, colStride, dtype, 1, rows,
+              cols, ptr<void>(q), qStride, ptr<void>(scales), device,
+              toStream(stream));
+        } else {
+          hip::launchQuantizeFp8(
+              ptr<const void>(x), rowStride, colStride, dtype, rows, cols,
+              ptr<void>(q), qStride, ptr<void>(scales), device,
+              toStream(stream));
+        }
       });
 
   m.def(

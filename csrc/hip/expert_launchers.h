@@ -19,6 +19,7 @@ struct ExpertLaunchers {
   decltype(&launchExpertCombine) combine;
   decltype(&launchExpertCombineBackward) combineBackward;
   decltype(&launchQuantizeFp8) quantize;
+  decltype(&launchQuantizeFp8Tiles) quantizeTiles;
   decltype(&launchFp8Matmul) matmul;
   decltype(&launchFp8WeightGrad) weightGrad;
 };

@@ -19,9 +19,8 @@ namespace hip {
 constexpr int kFp8Block = 128; // elements along a row that share a scale
 
 // q[r, c] = e4m3(x[r, c] / 2^e) and the scales' e of each 1 x 128 block
-// (scales [rows, ceil(cols / 128)]), or of each 128 x 128 tile where `tile`
-// (scales [ceil(rows / 128), ceil(cols / 128)]). x has any strides. q's rows
-// are qStride bytes apart, a multiple of 16; the bytes between are zeros.
+// (scales [rows, ceil(cols / 128)]). x has any strides. q's rows are qStride
+// bytes apart, a multiple of 16; the bytes between are zeros.
 void launchQuantizeFp8(
     const void* x,
     int64_t rowStride,
@@ -29,7 +28,24 @@ void launchQuantizeFp8(
     DType dtype,
     int64_t rows,
     int64_t cols,
-    bool tile,
+    void* q,
+    int64_t qStride,
+    void* scales,
+    int device,
+    hipStream_t stream);
+
+// The same with a scale for each 128 x 128 tile of each expert's matrix:
+// q [experts, rows, qStride], scales [experts, ceil(rows / 128),
+// ceil(cols / 128)].
+void launchQuantizeFp8Tiles(
+    const void* x,
+    int64_t expertStride,
+    int64_t rowStride,
+    int64_t colStride,
+    DType dtype,
+    int64_t experts,
+    int64_t rows,
+    int64_t cols,
     void* q,
     int64_t qStride,
     void* scales,

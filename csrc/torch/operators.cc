@@ -320,36 +320,35 @@ packFp8(const Tensor& tokens, const Tensor& position, int64_t stream) {
   return {q, scales};
 }
 
-void quantizeOne(
-    const Tensor& x,
-    bool tile,
-    const Tensor& q,
-    int64_t pitch,
-    const Tensor& scales,
-    int64_t stream) {
-  if (x.numel() != 0) {
-    launchers.quantize(
-        x.const_data_ptr(), x.stride(0), x.stride(1), typeOf(x), x.size(0),
-        x.size(1), tile, q.mutable_data_ptr(), pitch,
-        scales.mutable_data_ptr(), x.get_device(), toStream(stream));
-  }
-}
-
 std::pair<Tensor, Tensor>
 quantize(const Tensor& x, bool tile, int64_t stream) {
   const int64_t rows = x.size(-2);
   const int64_t cols = x.size(-1);
-  if (x.dim() == 2) {
-    auto [q, pitch] = fp8Rows({rows}, cols, x);
-    Tensor scales =
-        fp8Scales({tile ? blocksOf(rows) : rows, blocksOf(cols)}, x);
-    quantizeOne(x, tile, q, pitch, scales, stream);
+  const bool many = x.dim() == 3;
+  std::vector<int64_t> shape;
+  if (many) {
+    shape.push_back(x.size(0));
+  }
+  std::vector<int64_t> blocks = shape;
+  shape.push_back(rows);
+  blocks.push_back(tile ? blocksOf(rows) : rows);
+  blocks.push_back(blocksOf(cols));
+  auto [q, pitch] = fp8Rows(std::move(shape), cols, x);
+  Tensor scales = fp8Scales(blocks, x);
+  if (x.numel() == 0) {
     return {q, scales};
   }
-  auto [q, pitch] = fp8Rows({x.size(0), rows}, cols, x);
-  Tensor scales = fp8Scales({x.size(0), blocksOf(rows), blocksOf(cols)}, x);
-  for (int64_t e = 0; e < x.size(0); e++) {
-    quantizeOne(x[e], true, q[e], pitch, scales[e], stream);
+  if (tile) {
+    launchers.quantizeTiles(
+        x.const_data_ptr(), many ? x.stride(0) : 0, x.stride(-2),
+        x.stride(-1), typeOf(x), many ? x.size(0) : 1, rows, cols,
+        q.mutable_data_ptr(), pitch, scales.mutable_data_ptr(),
+        x.get_device(), toStream(stream));
+  } else {
+    launchers.quantize(
+        x.const_data_ptr(), x.stride(0), x.stride(1), typeOf(x), rows, cols,
+        q.mutable_data_ptr(), pitch, scales.mutable_data_ptr(),
+        x.get_device(), toStream(stream));
   }
   return {q, scales};
 }

@@ -538,12 +538,24 @@ def test_quantize_extremes():
     assert torch.isnan(q.float().cpu()[6, 5])
 
 
-def test_quantize_of_experts():
-    w = torch.randn(3, 200, 300).cuda()
-    q, s = ex.quantize_fp8(w, tile=True)
-    assert q.shape == w.shape and s.shape == (3, 2, 3)
-    for e in range(3):
-        same_quant((q[e], s[e]), quant_ref(w[e].cpu(), 128))
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r,c", [(1, 1), (64, 136), (129, 128), (200, 300),
+                                 (136, 264)])
+def test_quantize_of_experts(r, c, dtype):
+    x = some(3 * r, c, dtype).view(3, r, c)
+    refs = [quant_ref(x[e], 128) for e in range(3)]
+    g = x.cuda()
+    wide = torch.zeros(3, r + 1, c + 3, dtype=dtype, device="cuda")
+    wide[:, 1:, 2:2 + c] = g
+    for w in (g, g.transpose(1, 2).contiguous().transpose(1, 2),
+              wide[:, 1:, 2:2 + c], g.permute(1, 2, 0).contiguous().permute(
+                  2, 0, 1), g[:, None].expand(3, 2, r, c)[:, 1]):
+        q, s = ex.quantize_fp8(w, tile=True)
+        assert q.shape == w.shape and s.shape == (3, nb(r), nb(c))
+        for e in range(3):
+            same_quant((q[e], s[e]), refs[e])
+    q, s = ex.quantize_fp8(g[:1].expand(4, r, c), tile=True)
+    same_quant((q[3], s[3]), refs[0])
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
