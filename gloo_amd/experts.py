@@ -11,8 +11,10 @@
 runs the whole way over a process group. All operators are hand-written HIP
 kernels (csrc/hip/experts.hip, csrc/hip/fp8.hip, called by csrc/torch) that
 run asynchronously on the current stream of their tensors' device, allocate
-with torch's allocator and may be captured into a graph. Tensors have to be on a GPU; wrong arguments
-raise ValueError before anything is launched.
+with torch's allocator and may be captured into a graph (a backward pass only
+while no autograd graph of the same leaves from outside the capture is alive,
+as torch has it). Tensors have to be on a GPU; wrong arguments raise
+ValueError before anything is launched.
 
 8-bit values are torch.float8_e4m3fn. Their scales are powers of two
 (torch.float8_e8m0fnu): the least that brings a block's largest value to 448
@@ -415,9 +417,10 @@ class ExpertExchange:
     tokens by expert, the counts travel as a small alltoall of host tensors
     (so that dispatch waits for the GPU once), the rows as one alltoall with
     split sizes, and what arrives from the ranks is packed by expert again.
-    All ranks call both methods, ranks without tokens too. With bf16 rows and
-    the like the whole way is differentiable; with `fp8` the rows and their
-    scales travel in 8 bits.
+    All ranks call both methods, ranks without tokens too, with rows of one
+    length and type. With 16- or 32-bit rows the whole way is differentiable,
+    and all ranks run its backward pass; with `fp8` the rows and their scales
+    travel in 8 bits.
     """
 
     def __init__(self, num_experts, group=None):
@@ -446,6 +449,9 @@ class ExpertExchange:
         ExpertBatch with this rank's experts' rows."""
         _tensor(x, "x", 2, _FLOATS)
         _tensor(experts, "experts", 2, (torch.int32,), x)
+        if x.shape[1] < 1:
+            raise ValueError(f"x: rows of one element at least, got "
+                             f"{tuple(x.shape)}")
         if experts.shape[0] != x.shape[0] or experts.shape[1] < 1:
             raise ValueError(f"experts: one row a token, got "
                              f"{tuple(experts.shape)} for {x.shape[0]}")

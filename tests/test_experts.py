@@ -224,6 +224,8 @@ def test_exchange_refuses():
         ids = torch.zeros(4, 2, dtype=torch.int32)
         with pytest.raises(ValueError, match="one row a token"):
             exchange.dispatch(torch.zeros(5, 8), ids)
+        with pytest.raises(ValueError, match="one element"):
+            exchange.dispatch(torch.zeros(4, 0), ids)
         with pytest.raises(ValueError, match="on a GPU"):
             exchange.dispatch(torch.zeros(4, 8), ids)
         return True
