@@ -121,7 +121,9 @@ __global__ __launch_bounds__(256) void quantizeRowsKernel(
 
 // Any strides, and adjacent rows above all: a transposed matrix. A workgroup
 // takes 256 bytes of each of 128 columns through LDS, so that lanes run along
-// the rows for loads and scales and along the columns for stores.
+// the rows for loads and scales, and the bytes through LDS again, so that
+// they run along the columns for stores. 16384 x 4096 bf16, transposed, 201 MB,
+// take 47 us, 4.3 TB/s (57 with bytes stored by lanes that run along the rows).
 template <typename T, bool kVec>
 __global__ __launch_bounds__(256) void quantizeColumnsKernel(
     const T* __restrict__ x,
@@ -132,8 +134,10 @@ __global__ __launch_bounds__(256) void quantizeColumnsKernel(
   constexpr int kRows = 16 * kSize; // 256 bytes
   constexpr int kParts = 256 / kRows; // lanes that share a row
   constexpr int kEach = kQuant / kParts; // columns of one of them
+  constexpr int kWords = kQuant / 4 + 1; // of a row of bytes in LDS
   __shared__ Vec16<T> tile[kQuant][16];
   __shared__ uint32_t most[kParts][kRows];
+  auto* bytes = reinterpret_cast<uint32_t*>(tile); // [kRows][kWords]
   const int64_t row0 = static_cast<int64_t>(blockIdx.x) * kRows;
   const int64_t col0 = static_cast<int64_t>(blockIdx.y) * kQuant;
   const int chunk = threadIdx.x % 16;
@@ -172,21 +176,28 @@ __global__ __launch_bounds__(256) void quantizeColumnsKernel(
   for (int i = 0; i < kParts; i++) {
     amax = maxBits(amax, most[i][r]);
   }
-  const int64_t row = row0 + r;
-  if (row >= p.rows) {
-    return;
-  }
   const uint32_t byte = fp8ScaleByte(amax);
   const float inv = fp8InverseScale(byte);
-  const int64_t at = col0 + part * kEach;
 #pragma unroll
-  for (int i = 0; i < kEach / 16; i++) {
-    if (at + i * 16 + 16 <= p.qStride) {
-      storeFp8<16>(q + row * p.qStride + at + i * 16, v + i * 16, inv);
-    }
+  for (int i = 0; i < kEach / 4; i++) {
+    bytes[r * kWords + part * (kEach / 4) + i] = fp8Pack4(
+        v[i * 4] * inv, v[i * 4 + 1] * inv, v[i * 4 + 2] * inv,
+        v[i * 4 + 3] * inv);
   }
-  if (part == 0) {
-    scales[row * gridDim.y + blockIdx.y] = static_cast<uint8_t>(byte);
+  if (part == 0 && row0 + r < p.rows) {
+    scales[(row0 + r) * gridDim.y + blockIdx.y] = static_cast<uint8_t>(byte);
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kRows / 32; i++) {
+    const int at = i * 32 + threadIdx.x / 8;
+    const int64_t row = row0 + at;
+    const int64_t col = col0 + threadIdx.x % 8 * 16;
+    if (row < p.rows && col + 16 <= p.qStride) {
+      const uint32_t* w = bytes + at * kWords + threadIdx.x % 8 * 4;
+      *reinterpret_cast<uint4*>(q + row * p.qStride + col) =
+          make_uint4(w[0], w[1], w[2], w[3]);
+    }
   }
 }
 
