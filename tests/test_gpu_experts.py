@@ -814,6 +814,58 @@ def test_results_larger_than_the_caches(n, out):
         assert torch.equal(got[i], (a[:, part] @ b[:, part].t()).to(out))
 
 
+def whole_numbers(gen, *shape):
+    """Operands whose products' sums are exact in 32 bits, with scales of 1."""
+    x = torch.randint(-3, 4, shape, generator=gen, device="cuda").float()
+    scales = shape[:-1] + (nb(shape[-1]),)
+    return x, x.to(F8), torch.ones(scales, device="cuda").to(E8)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("inner", [128, 200, 256, 384, 656, 1152])
+@pytest.mark.parametrize("n", [5200, 2570, 1300, 700, 260])
+def test_tiles_of_a_product(n, inner, out):
+    """From the smallest tiles to the largest, with every number of blocks
+    from one to five, of experts with and without rows."""
+    gen = torch.Generator(device="cuda").manual_seed(n + inner)
+    at = [0, 300, 300, 301, 1000, 1192, 1320, 2344, 2600, 2800]
+    rows = at[-1] + 30
+    a, qa, sa = whole_numbers(gen, rows, inner)
+    b, qb, _ = whole_numbers(gen, len(at) - 1, n, inner)
+    sb = torch.ones(len(at) - 1, nb(n), nb(inner), device="cuda").to(E8)
+    got = ex.fp8_matmul(qa, sa, qb, sb, dtype=out,
+                        offsets=torch.tensor(at, dtype=torch.int32).cuda())
+    for e in range(len(at) - 1):
+        part = slice(at[e], at[e + 1])
+        assert torch.equal(got[part], (a[part] @ b[e].t()).to(out)), e
+    assert (got[at[-1]:] == 0).all()
+    got = ex.fp8_matmul(qa, sa, qb[0], sb[0], dtype=out)
+    assert torch.equal(got, (a @ b[0].t()).to(out))
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n", [(2064, 2308), (1000, 1100), (600, 700),
+                                 (300, 260)])
+@pytest.mark.parametrize("at", [
+    [0, 8200], [0, 8192], [0, 130, 130, 777, 1300],
+    [0, 127, 128, 129, 384, 900, 901, 1800, 4000], [0, 512, 1024, 1408],
+])
+def test_tiles_of_a_weight_gradient(at, m, n, out):
+    """The same: experts of one block and of many, whose first and last
+    blocks are their neighbours' too."""
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    rows = at[-1]
+    a, qa, sa = whole_numbers(gen, m, rows)
+    b, qb, sb = whole_numbers(gen, n, rows)
+    got = ex.fp8_weight_grad(
+        qa, sa, qb, sb, dtype=out,
+        offsets=torch.tensor(at, dtype=torch.int32).cuda())
+    for e in range(len(at) - 1):
+        part = slice(at[e], at[e + 1])
+        assert torch.equal(got[e],
+                           (a[:, part] @ b[:, part].t()).to(out)), e
+
+
 def test_single_rows_of_any_stride():
     gen = torch.Generator().manual_seed(6)
     a, sa = operand((1, 512), (1, 4), gen)
