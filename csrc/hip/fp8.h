@@ -68,8 +68,8 @@ struct Fp8ProductArgs {
   void* out = nullptr; // [rows, n]
   DType dtype = DType::BF16; // of out: F32, F16 or BF16
 };
-// out[r] = b[e] a[r] for the rows of each expert; zeros for the rows behind
-// the last expert's.
+// out[r] = b[e] a[r] for the rows of each expert; zeros for rows before the
+// first expert's and behind the last one's.
 void launchFp8Matmul(
     const Fp8ProductArgs& args,
     int device,

@@ -357,8 +357,8 @@ struct ProductShape {
   bool stream; // results are stored past the caches
 };
 
-// Part of an expert's rows: [begin, end) of `of`, kBM at most. of ==
-// experts: the rows behind the last one.
+// Part of an expert's rows: [begin, end) of `of`. of == experts: the rows
+// behind the last one's, experts + 1: those before the first one's.
 struct RowTile {
   int of;
   int64_t begin;
@@ -384,7 +384,7 @@ __device__ inline int64_t clampOffset(
   return v < 0 ? 0 : (v > rows ? rows : v);
 }
 
-// Rows [begin, end) of expert e, or those behind the last one.
+// Rows [begin, end) of expert e, or those of none (see RowTile).
 __device__ inline void rowsOf(
     const ProductShape& p,
     int e,
@@ -395,6 +395,8 @@ __device__ inline void rowsOf(
   if (e <= p.experts) {
     begin = clampOffset(p.offsets, e, p.m);
     end = e < p.experts ? clampOffset(p.offsets, e + 1, p.m) : p.m;
+  } else if (e == p.experts + 1) {
+    end = clampOffset(p.offsets, 0, p.m);
   }
 }
 
@@ -415,7 +417,7 @@ __device__ inline int countTiles(const ProductShape& p, int size) {
     return static_cast<int>((p.m + size - 1) / size);
   }
   int base = 0;
-  for (int from = 0; from <= p.experts; from += kWave) {
+  for (int from = 0; from < p.experts + 2; from += kWave) {
     int64_t begin;
     int64_t end;
     rowsOf(p, from + static_cast<int>(threadIdx.x) % kWave, begin, end);
@@ -437,7 +439,7 @@ __device__ inline RowTile findTile(
     return RowTile{begin < p.m ? 0 : -1, begin, end};
   }
   int base = 0;
-  for (int from = 0; from <= p.experts; from += kWave) {
+  for (int from = 0; from < p.experts + 2; from += kWave) {
     int64_t begin;
     int64_t end;
     rowsOf(p, from + static_cast<int>(threadIdx.x) % kWave, begin, end);
@@ -1350,7 +1352,7 @@ matmulKernel(ProductShape p, O* __restrict__ out) {
   job.n0 = static_cast<int64_t>(at.n) * T::kN;
   job.k0 = 0;
   job.k1 = p.inner;
-  if (tile.of == p.experts) {
+  if (p.offsets != nullptr && tile.of >= p.experts) {
     job.k1 = 0; // no expert's rows: zeros
   } else {
     job.b.p += tile.of * p.bExpertStride;
@@ -1382,7 +1384,7 @@ __global__ __launch_bounds__(kWaves * kWave) void fewRowsKernel(
     rowsOf(p, e, begin, end);
   }
   const bool whole = p.n % 4 == 0;
-  if (e == p.experts) { // rows behind the last expert's: zeros
+  if (p.offsets != nullptr && e >= p.experts) { // no expert's: zeros
     const float zero[4] = {0, 0, 0, 0};
     for (int64_t i = threadIdx.x; i < (end - begin) * 4;
          i += kWaves * kWave) {
@@ -1538,10 +1540,10 @@ constexpr int64_t kEnough = 192;
 constexpr int kShort = 32;
 
 // Tiles of rows, at most: every expert's last one may be a part of one, and
-// so may that of the rows behind the last expert.
+// so may those of the rows of no expert, before the first and behind the last.
 template <typename T>
 int64_t tilesOf(T, const ProductShape& p, bool grouped) {
-  return grouped ? p.m / T::kM + std::min<int64_t>(p.experts + 1, p.m)
+  return grouped ? p.m / T::kM + std::min<int64_t>(p.experts + 2, p.m)
                  : (p.m + T::kM - 1) / T::kM;
 }
 
@@ -1577,7 +1579,7 @@ void checkProduct(const ProductShape& p) {
   GA_ENFORCE_LE(p.n, INT32_MAX);
   GA_ENFORCE_LE(p.inner, INT32_MAX);
   GA_ENFORCE_GT(p.experts, 0);
-  GA_ENFORCE_LT(p.experts, 65535);
+  GA_ENFORCE_LT(p.experts, 65534);
   GA_ENFORCE_GE(p.aStride, 0);
   GA_ENFORCE_GE(p.bStride, 0);
 }
@@ -1753,7 +1755,7 @@ void launchFp8Matmul(
         constexpr int kWaves = decltype(waves)::value;
         const dim3 grid(
             groupsOf((p.n + 15) / 16, kWaves * kWave),
-            a.offsets != nullptr ? p.experts + 1 : 1);
+            a.offsets != nullptr ? p.experts + 2 : 1);
         hipLaunchKernelGGL(
             (fewRowsKernel<O, kRows, kWaves>), grid, dim3(kWaves * kWave), 0,
             stream, p, static_cast<O*>(a.out));

@@ -300,8 +300,8 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
     [rows, n] in `dtype` (float32, float16 or bfloat16), added up in float32
     and rounded once. With `offsets` (int32 [experts + 1], a plan's) b and
     b_scale have a leading dimension for experts, and rows offsets[e] to
-    offsets[e + 1] are multiplied by b[e]; rows behind the last expert's are
-    zeros. The data gradient is the same product with the weights'
+    offsets[e + 1] are multiplied by b[e]; rows before the first expert's (some
+    of a plan's experts will do) and behind the last one's are zeros. The data gradient is the same product with the weights'
     transposed copy; `fp8_weight_grad` is the other one."""
     if not isinstance(a, torch.Tensor) or a.dim() != 2:
         raise ValueError("a: a tensor of 2 dimensions is needed")

@@ -844,6 +844,28 @@ def test_tiles_of_a_product(n, inner, out):
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("at,rows,n", [
+    ([2, 3, 5], 6, 70), ([40, 90, 90, 100], 130, 300), ([7, 7], 7, 40),
+    ([300, 1000, 2200], 2900, 5200), ([129, 300] + [300] * 90, 400, 130),
+])
+def test_rows_of_some_experts(at, rows, n, out):
+    """Offsets that begin behind the first row: those rows are zeros too."""
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    a, qa, sa = whole_numbers(gen, rows, 300)
+    b, qb, _ = whole_numbers(gen, len(at) - 1, n, 300)
+    sb = torch.ones(len(at) - 1, nb(n), 3, device="cuda").to(E8)
+    off = torch.tensor(at, dtype=torch.int32).cuda()
+    ref = torch.zeros(rows, n, device="cuda")
+    for e in range(len(at) - 1):
+        part = slice(at[e], at[e + 1])
+        ref[part] = a[part] @ b[e].t()
+    # what the result's memory held before
+    torch.full((rows, n), 7.0, dtype=out, device="cuda")
+    got = ex.fp8_matmul(qa, sa, qb, sb, dtype=out, offsets=off)
+    assert torch.equal(got, ref.to(out))
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m,n", [(2064, 2308), (1000, 1100), (600, 700),
                                  (300, 260)])
 @pytest.mark.parametrize("at", [
