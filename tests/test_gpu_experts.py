@@ -1071,6 +1071,109 @@ def test_training_step_captured():
             assert torch.equal(a, b)
 
 
+def test_gradients_of_one_input_alone():
+    """Where only rows, or only weights, want a gradient; gradients of any
+    strides; a graph that is kept and run again; recomputation."""
+    from torch.utils.checkpoint import checkpoint
+    gen = torch.Generator().manual_seed(11)
+    t, k, h = 30, 3, 72
+    p = ex.plan(ids_of(t, k, 8, gen, 0.2).cuda(), 8)
+    rows = torch.randn(t * k, h, generator=gen).cuda()
+    w = torch.rand(t, k, generator=gen).cuda()
+    g = torch.randn(h, t, generator=gen).cuda().t()  # not contiguous
+    r, v = rows.clone().requires_grad_(), w.clone().requires_grad_()
+    out = ex.combine(r, p, v)
+    both = torch.autograd.grad(out, (r, v), g, retain_graph=True)
+    again = torch.autograd.grad(out, (r, v), g)
+    alone = (torch.autograd.grad(ex.combine(r, p, w), r, g)[0],
+             torch.autograd.grad(ex.combine(rows, p, v), v, g)[0])
+    lazy = torch.autograd.grad(
+        checkpoint(lambda a, b: ex.combine(a, p, b), r, v,
+                   use_reentrant=False), (r, v), g)
+    for other in (again, alone, lazy):
+        for a, b in zip(both, other):
+            assert torch.equal(a, b)
+    x = torch.randn(t, h, generator=gen).cuda().requires_grad_()
+    one = torch.ones((), device="cuda").expand(t * k, h)
+    dx, = torch.autograd.grad(ex.pack(x, p), x, one)
+    copies = (p.position >= 0).sum(1, keepdim=True)
+    assert torch.equal(dx, copies.float().expand(t, h))
+
+
+def test_two_graphs_that_share_their_memory():
+    """Captured into one pool, replayed in turn with eager calls between."""
+    gen = torch.Generator().manual_seed(12)
+    t, k, e, h = 9000, 8, 64, 24  # several chunks of ids
+    inputs = []
+    for _ in range(2):
+        x = torch.randn(t, h, generator=gen).cuda()
+        inputs.append([x, ids_of(t, k, e, gen).cuda()])
+
+    def step(x, ids):
+        p = ex.plan(ids, e)
+        return p.position, ex.combine(ex.pack(x, p), p)
+
+    step(*inputs[0])
+    stream, pool, graphs, outs = torch.cuda.Stream(), None, [], []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(stream):
+        for i in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, pool=pool, stream=stream):
+                outs.append(step(*inputs[i]))
+            pool = graph.pool()
+            graphs.append(graph)
+    torch.cuda.synchronize()
+    for turn in range(3):
+        for x, ids in inputs:
+            x.copy_(torch.randn(t, h, generator=gen))
+            ids.copy_(ids_of(t, k, e, gen))
+        refs = [[v.clone() for v in step(*pair)] for pair in inputs]
+        for i in (0, 1) if turn % 2 else (1, 0):
+            graphs[i].replay()
+            for a, b in zip(outs[i], refs[i]):
+                assert torch.equal(a, b)
+
+
+def test_calls_from_threads():
+    """Four threads, each on a stream of its own."""
+    import threading
+    gen = torch.Generator().manual_seed(13)
+    t, e, h, n = 300, 16, 256, 192
+    w, ws = ex.quantize_fp8(torch.randn(e, n, h, generator=gen).cuda(),
+                            tile=True)
+    data = [(torch.randn(t, e, generator=gen).cuda(),
+             torch.randn(t, h, generator=gen).cuda().bfloat16())
+            for _ in range(4)]
+
+    def step(z, x):
+        z = z.detach().requires_grad_()
+        gate, ids = ex.route(z, 4)
+        p = ex.plan(ids, e)
+        y = ex.fp8_matmul(*ex.pack_fp8(x, p), w, ws, p.offsets)
+        out = ex.combine(y, p, gate)
+        return out.detach(), torch.autograd.grad(out.float().sum(), z)[0]
+
+    refs = [step(*pair) for pair in data]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(10):
+                got = step(*data[i])
+                torch.cuda.current_stream().synchronize()
+                if not all(map(torch.equal, got, refs[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for thread in threads:
+        thread.start()
+    for thread in threads:
+        thread.join()
+    assert not wrong
+
+
 def test_raw_entry_points():
     """The same kernels by device pointers, on the null stream."""
     gen = torch.Generator().manual_seed(15)
