@@ -40,8 +40,8 @@ struct RouteArgs {
 };
 void launchRoute(const RouteArgs& args, int device, hipStream_t stream);
 
-// dlogits [tokens, experts] (contiguous, the logits' type) of `grad`
-// [tokens, k]; args.ids are the forward pass's.
+// dlogits [tokens, experts] (contiguous, the logits' type, begins on 16
+// bytes) of `grad` [tokens, k]; args.ids are the forward pass's.
 void launchRouteBackward(
     const RouteArgs& args,
     const float* grad,

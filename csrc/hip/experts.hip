@@ -1116,6 +1116,8 @@ void launchRouteBackward(
     int device,
     hipStream_t stream) {
   RouteShape p = checkRoute(a);
+  GA_ENFORCE(
+      aligned16(dlogits), "route: the gradient must begin on 16 bytes");
   if (p.tokens == 0) {
     return;
   }

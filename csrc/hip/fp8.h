@@ -65,7 +65,7 @@ struct Fp8ProductArgs {
   int64_t n = 0;
   int64_t inner = 0;
   int experts = 1;
-  void* out = nullptr; // [rows, n]
+  void* out = nullptr; // [rows, n], begins on 16 bytes
   DType dtype = DType::BF16; // of out: F32, F16 or BF16
 };
 // out[r] = b[e] a[r] for the rows of each expert; zeros for rows before the
@@ -87,7 +87,7 @@ struct Fp8WeightGradArgs {
   int64_t n = 0;
   int64_t rows = 0;
   int experts = 1;
-  void* out = nullptr; // [experts, m, n]
+  void* out = nullptr; // [experts, m, n], begins on 16 bytes
   DType dtype = DType::F32;
 };
 // out[e] = sum over the expert's rows r of dy[:, r] x[:, r]^T.

@@ -1726,6 +1726,7 @@ void launchFp8Matmul(
   p.experts = a.experts;
   checkProduct(p);
   GA_ENFORCE(a.offsets != nullptr || a.experts == 1);
+  GA_ENFORCE(aligned16(a.out), "fp8_matmul: out must begin on 16 bytes");
   if (p.m == 0) {
     return;
   }
@@ -1815,6 +1816,8 @@ void launchFp8WeightGrad(
   checkProduct(p);
   GA_ENFORCE_GT(a.m, 0);
   GA_ENFORCE(a.offsets != nullptr || a.experts == 1);
+  GA_ENFORCE(
+      aligned16(a.out), "fp8_weight_grad: out must begin on 16 bytes");
   DeviceGuard guard(device);
   p.aWhole = whole16(p.a, p.aStride);
   p.bWhole = whole16(p.b, p.bStride);

@@ -179,6 +179,13 @@ def test_launchers_check_for_themselves():
     with pytest.raises(ga.EnforceNotMet):
         ga._C.hip_fp8_weight_grad(0, 128, 0, 0, 128, 0, 0, 4, 0, 8, 1, 0, f,
                                   0, s)
+    for out in (4, 8):  # results on no border of 16
+        with pytest.raises(ga.EnforceNotMet, match="16 bytes"):
+            ga._C.hip_fp8_matmul(0, 128, 0, 0, 128, 0, 0, 0, 4, 8, 128, 1,
+                                 out, f, 0, s)
+        with pytest.raises(ga.EnforceNotMet, match="16 bytes"):
+            ga._C.hip_fp8_weight_grad(0, 128, 0, 0, 128, 0, 0, 4, 4, 8, 1,
+                                      out, f, 0, s)
 
 
 def test_exchange_of_rows_between_ranks():
