@@ -822,7 +822,7 @@ def whole_numbers(gen, *shape):
 
 
 @pytest.mark.parametrize("out", [torch.float32, torch.bfloat16])
-@pytest.mark.parametrize("inner", [128, 200, 256, 384, 656, 1152])
+@pytest.mark.parametrize("inner", [128, 200, 256, 384, 656, 1152, 2192])
 @pytest.mark.parametrize("n", [5200, 2570, 1300, 700, 260])
 def test_tiles_of_a_product(n, inner, out):
     """From the smallest tiles to the largest, with every number of blocks
