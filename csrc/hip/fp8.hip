@@ -812,20 +812,7 @@ struct Stager {
     }
   }
 
-  // Zeros in place of what loadDirect brought and does not count.
-  __device__ void mask(int64_t k, uint4* lds) const {
-#pragma unroll 1
-    for (int i = 0; i < kEach; i++) {
-      const int chunk = i * kThreads + threadIdx.x;
-      const int c = chunkOf(chunk / kChunks, chunk % kChunks);
-      const int64_t at = k + c * 16;
-      if (at < lo || at + 16 > hi) {
-        lds[chunk] = maskOf(lds[chunk], at, lo, hi);
-      }
-    }
-  }
-
-  // The same for any bytes, through masks.
+  // Bytes k on through masks.
   __device__ void loadMasked(int64_t k, uint4* lds) const {
 #pragma unroll 1
     for (int i = 0; i < kEach; i++) {
@@ -1059,12 +1046,7 @@ struct Product {
     }
   }
 
-  // Exact: while one piece is multiplied the next one is converted, which the
-  // groups ask of the compiler: left alone it converts first and multiplies
-  // then, and the matrix unit waits.
-  __device__ void stepExact(const Half (&f)[2]) {
-    float fa[TM];
-    float fb[TN];
+  __device__ void scales(float (&fa)[TM], float (&fb)[TN]) const {
 #pragma unroll
     for (int j = 0; j < TM; j++) {
       fa[j] = scaleOf(sa[j]);
@@ -1073,6 +1055,26 @@ struct Product {
     for (int i = 0; i < TN; i++) {
       fb[i] = scaleOf(sb[i]);
     }
+  }
+
+  __device__ void add(const Piece& f) {
+#pragma unroll
+    for (int i = 0; i < TN; i++) {
+#pragma unroll
+      for (int j = 0; j < TM; j++) {
+        acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
+            f.b[i], f.a[j], acc[i][j], 0, 0, 0);
+      }
+    }
+  }
+
+  // Exact: while one piece is multiplied the next one is converted, which the
+  // groups ask of the compiler: left alone it converts first and multiplies
+  // then, and the matrix unit waits.
+  __device__ void stepExact(const Half (&f)[2]) {
+    float fa[TM];
+    float fb[TN];
+    scales(fa, fb);
     Piece piece[2];
     convert(f[0], 0, fa, fb, piece[0]);
     __builtin_amdgcn_sched_barrier(0);
@@ -1081,14 +1083,7 @@ struct Product {
       if (u < 7) {
         convert(f[(u + 1) / 4], (u + 1) % 4, fa, fb, piece[(u + 1) % 2]);
       }
-#pragma unroll
-      for (int i = 0; i < TN; i++) {
-#pragma unroll
-        for (int j = 0; j < TM; j++) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-              piece[u % 2].b[i], piece[u % 2].a[j], acc[i][j], 0, 0, 0);
-        }
-      }
+      add(piece[u % 2]);
 #pragma unroll
       for (int i = 0; i < TN * TM; i++) {
         __builtin_amdgcn_sched_group_barrier(0x8, 1, 0); // one product
@@ -1114,6 +1109,55 @@ struct Product {
         add(f);
       }
     }
+  }
+
+  // A block of which only bytes [k0, k1) count, zeros in place of the others:
+  // they may be NaN. Half a block that has none is left out.
+  __device__ void
+  stepEdge(const uint4* la, const uint4* lb, const int* ls, int k) {
+    readScales(ls);
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const int first = k + h * 64;
+      if (first + 64 <= job.k0 || first >= job.k1) {
+        continue;
+      }
+      Half f;
+      read(la, lb, h, f);
+      const int own = first + lane / 32 * 32;
+      Int8 mask;
+#pragma unroll
+      for (int w = 0; w < 8; w++) {
+        mask[w] = bytesFrom(job.k0 - own - w * 4) &
+            ~bytesFrom(job.k1 - own - w * 4);
+      }
+#pragma unroll
+      for (int j = 0; j < TM; j++) {
+        f.a[j].v &= mask;
+      }
+#pragma unroll
+      for (int i = 0; i < TN; i++) {
+        f.b[i].v &= mask;
+      }
+      if constexpr (kExact) {
+        float fa[TM];
+        float fb[TN];
+        scales(fa, fb);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+          Piece piece;
+          convert(f, i, fa, fb, piece);
+          add(piece);
+        }
+      } else {
+        add(f);
+      }
+    }
+  }
+
+  // The bytes of a word from the n-th on.
+  static __device__ int bytesFrom(int n) {
+    return n <= 0 ? -1 : (n >= 4 ? 0 : -1 << n * 8);
   }
 
   // A ring of three stages of LDS, two on their way while one is multiplied,
@@ -1150,8 +1194,9 @@ struct Product {
     const int last =
         uniform(static_cast<int>((job.k1 + kQuant - 1) / kQuant));
     // Blocks that lie within the rows, [first, direct), are loaded directly.
-    // An expert's first and last one may hold bytes of its neighbours: those
-    // come behind the others, [whole0, whole1), and are masked.
+    // An expert's first and last one in a weight gradient may hold bytes of
+    // its neighbours: those come behind the others, [whole0, whole1), and are
+    // masked.
     const int full = static_cast<int>(job.a.inner / kQuant);
     const int direct = uniform(
         a.direct && b.direct ? (last < full ? last : full) : first);
@@ -1182,14 +1227,12 @@ struct Product {
       const auto rest = [&](int t, uint4* la, uint4* lb, const int* ls,
                             auto live) {
         if (t < total) {
-          if (t >= whole) {
-            const int64_t k = static_cast<int64_t>(nth(t)) * kQuant;
-            a.mask(k, la);
-            b.mask(k, lb);
-            arrived<63>();
-          }
           if constexpr (decltype(live)::value) {
-            step(la, lb, ls);
+            if (!kWeightGrad || t < whole) {
+              step(la, lb, ls);
+            } else {
+              stepEdge(la, lb, ls, nth(t) * kQuant);
+            }
           }
         }
       };
