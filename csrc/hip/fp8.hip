@@ -1577,9 +1577,8 @@ constexpr int64_t kEnough = 192;
 // A weight gradient of experts with few rows is done with a tile after a few
 // steps: two workgroups with small tiles on a compute unit, with two stages of
 // LDS each, store and multiply at the same time. 16 experts, 16384 x 4096 x
-// 2048 (about eight steps): 391 us against 445 with the large tile for fp32
-// results, 270 / 302 for bf16; 4 experts 355 / 350 and 242 / 246, one expert
-// behind.
+// 2048 (about eight steps): 367 us against 414 with the large tile for fp32
+// results, 250 / 290 for bf16; 4 experts, some 32 steps, are even.
 constexpr int kShort = 32;
 // So are products with fp32 results and a short inner dimension: 8192 x 4096 x
 // 512 48 us against 50, 8741 x 4096 x 512 of 8 experts 62 / 72, 16384 x 2048 x
