@@ -1526,27 +1526,34 @@ __global__ __launch_bounds__(kWaves * kWave) void fewRowsKernel(
   }
 }
 
-// A weight gradient's tiles take as long as their expert has rows. With few
-// experts a die would have one of them, and the dies would end one after the
-// other: each takes a part of every expert instead, if that is a band's worth
-// of tiles. Ragged rows, 16384 in all, fp32: 4 experts of 4096 x 2048 256 us
-// against 288, 8 of 1408 x 2048 108 / 145; from 16 on a die has several,
-// and its caches more of each: 16 of 4096 x 2048 403 / 405 (bf16 296 / 276),
-// 32 of 2048 x 1408 207 / 197.
-__host__ __device__ inline bool spread(int64_t tiles, int experts) {
-  return tiles >= kDies * kBand && experts < 2 * kDies;
+// A weight gradient's tiles take as long as their expert has rows, so that
+// dies with experts of their own would end one after the other. An expert's
+// tiles, if they are enough, are parted in eight or, with many experts, in
+// four, and the dies take the parts in turn. Ragged rows, 16384 in all, whole
+// experts and parts, in us: 4 experts of 4096 x 2048 274 / 244, 8 of 1408 x
+// 2048 134 / 103; 16 of 4096 x 2048 411 to 485 / 396 to 411, bf16 273 to 347 /
+// 276 to 288, 32 of 2048 x 1408 188 to 203 / 198 to 201, bf16 121 to 131 / 116
+// to 120, 64 of 1024 x 2048 242 to 250 / 224 to 226.
+__host__ __device__ inline int partsOf(int64_t tiles, int experts) {
+  return tiles < kDies * kBand ? 0 : (experts < 2 * kDies ? kDies : kDies / 2);
 }
 
-int64_t spreadTiles(int64_t tiles, int experts) {
-  return spread(tiles, experts)
-      ? (tiles + kDies - 1) / kDies * kDies * experts
-      : tiles * experts;
+int64_t weightTiles(int64_t tiles, int experts) {
+  const int parts = partsOf(tiles, experts);
+  if (parts == 0) {
+    return tiles * experts;
+  }
+  const int64_t units =
+      (static_cast<int64_t>(experts) * parts + kDies - 1) / kDies * kDies;
+  return (tiles + parts - 1) / parts * units;
 }
 
+// False: fewer tiles than workgroups.
 __device__ inline bool
 weightTileAt(const ProductShape& p, int tilesM, int& e, TileAt& at) {
   const int64_t tiles = static_cast<int64_t>(tilesM) * p.tilesN;
-  if (!spread(tiles, p.experts)) {
+  const int parts = partsOf(tiles, p.experts);
+  if (parts == 0) {
     if (!tileAt(tilesM * p.experts, p.tilesN, at)) {
       return false;
     }
@@ -1554,18 +1561,16 @@ weightTileAt(const ProductShape& p, int tilesM, int& e, TileAt& at) {
     at.m %= tilesM;
     return true;
   }
-  const int each = static_cast<int>((tiles + kDies - 1) / kDies);
+  const int each = static_cast<int>((tiles + parts - 1) / parts);
   const int id = blockIdx.x / kDies;
-  e = id / each;
-  if (e >= p.experts) {
+  const int unit = id / each * kDies + blockIdx.x % kDies;
+  e = unit / parts;
+  const int part = unit % parts;
+  const int64_t in = tiles * part / parts + id % each;
+  if (e >= p.experts || in >= tiles * (part + 1) / parts) {
     return false;
   }
-  const int part = (blockIdx.x + e) % kDies;
-  const int64_t at0 = tiles * part / kDies + id % each;
-  if (at0 >= tiles * (part + 1) / kDies) {
-    return false;
-  }
-  at = inBands(at0, tilesM, p.tilesN);
+  at = inBands(in, tilesM, p.tilesN);
   return true;
 }
 
@@ -1927,7 +1932,7 @@ void launchFp8WeightGrad(
       using T = decltype(tile);
       p.tilesN = static_cast<int>((p.n + T::kN - 1) / T::kN);
       const int64_t tiles =
-          spreadTiles((p.m + T::kM - 1) / T::kM * p.tilesN, p.experts);
+          weightTiles((p.m + T::kM - 1) / T::kM * p.tilesN, p.experts);
       hipLaunchKernelGGL(
           kernel, dim3(gridOf(tiles, T::kThreads)), dim3(T::kThreads), 0,
           stream, p, static_cast<O*>(a.out));

@@ -871,6 +871,7 @@ def test_rows_of_some_experts(at, rows, n, out):
 @pytest.mark.parametrize("at", [
     [0, 8200], [0, 8192], [0, 130, 130, 777, 1300],
     [0, 127, 128, 129, 384, 900, 901, 1800, 4000], [0, 512, 1024, 1408],
+    [0, 100, 100, 350, 351] + [400 + 97 * i for i in range(15)],
 ])
 def test_tiles_of_a_weight_gradient(at, m, n, out):
     """The same: experts of one block and of many, whose first and last
