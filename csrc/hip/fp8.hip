@@ -474,7 +474,8 @@ struct TileAt {
 };
 
 __device__ inline TileAt inBands(int64_t id, int tilesM, int tilesN) {
-  const int band = static_cast<int>(id / (static_cast<int64_t>(kBand) * tilesN));
+  const int band =
+      static_cast<int>(id / (static_cast<int64_t>(kBand) * tilesN));
   const int inBand =
       static_cast<int>(id - static_cast<int64_t>(band) * kBand * tilesN);
   const int left = tilesM - band * kBand;
@@ -1160,7 +1161,7 @@ struct Product {
 
   // The bytes of a word from the n-th on.
   static __device__ int bytesFrom(int n) {
-    return n <= 0 ? -1 : (n >= 4 ? 0 : -1 << n * 8);
+    return n <= 0 ? -1 : (n >= 4 ? 0 : static_cast<int>(~0u << n * 8));
   }
 
   // A ring of three stages of LDS, two on their way while one is multiplied,

@@ -35,6 +35,7 @@ _ops.set_launchers(_C.expert_launchers())
 FP8 = torch.float8_e4m3fn
 FP8_SCALE = torch.float8_e8m0fnu
 FP8_BLOCK = 128
+_FP8_EXPERTS = 65533  # of the 8-bit products
 _FLOATS = (torch.float32, torch.float16, torch.bfloat16)
 
 
@@ -301,8 +302,9 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
     and rounded once. With `offsets` (int32 [experts + 1], a plan's) b and
     b_scale have a leading dimension for experts, and rows offsets[e] to
     offsets[e + 1] are multiplied by b[e]; rows before the first expert's (some
-    of a plan's experts will do) and behind the last one's are zeros. The data gradient is the same product with the weights'
-    transposed copy; `fp8_weight_grad` is the other one."""
+    of a plan's experts will do) and behind the last one's are zeros. The data
+    gradient is the same product with the weights' transposed copy;
+    `fp8_weight_grad` is the other one."""
     if not isinstance(a, torch.Tensor) or a.dim() != 2:
         raise ValueError("a: a tensor of 2 dimensions is needed")
     if (not isinstance(b, torch.Tensor)
@@ -316,8 +318,9 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
     if b.shape[-1] != inner:
         raise ValueError(
             f"b: an inner dimension of {inner} is needed, got {b.shape[-1]}")
-    if n <= 0 or experts <= 0:
-        raise ValueError(f"b: got {tuple(b.shape)}")
+    if n <= 0 or not 0 < experts <= _FP8_EXPERTS:
+        raise ValueError(f"b: 1 to {_FP8_EXPERTS} experts, got "
+                         f"{tuple(b.shape)}")
     _fp8_operand(a, a_scale, "a", 2, (rows, _blocks(inner)))
     _fp8_operand(b, b_scale, "b", b.dim(),
                  tuple(b.shape[:-2]) + (_blocks(n), _blocks(inner)), a)
@@ -353,8 +356,9 @@ def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
     _fp8_operand(x, x_scale, "x", 2, (n, _blocks(rows)), dy)
     if offsets is not None and (
             not isinstance(offsets, torch.Tensor) or offsets.dim() != 1
-            or offsets.shape[0] < 2):
-        raise ValueError("offsets: [experts + 1] is needed")
+            or not 2 <= offsets.shape[0] <= _FP8_EXPERTS + 1):
+        raise ValueError(f"offsets: [experts + 1] is needed, for 1 to "
+                         f"{_FP8_EXPERTS} experts")
     _offsets(offsets, 0 if offsets is None else offsets.shape[0] - 1, dy)
     _gpu(dy, "fp8_weight_grad")
     return _ops.fp8_weight_grad(dy, dy_scale, x, x_scale, offsets, dtype,

@@ -112,6 +112,14 @@ def test_what_is_too_large_is_refused():
             call()
     with pytest.raises(ValueError, match="elements"):
         ex.pack(one.expand(4, 2 ** 23 + 1), _plan())
+    e = 65534
+    q, s, off = one.to(F8), one.to(E8), torch.zeros(e + 1, dtype=torch.int32)
+    with pytest.raises(ValueError, match="65533 experts"):
+        ex.fp8_matmul(q.expand(4, 128), s.expand(4, 1), q.expand(e, 8, 128),
+                      s.expand(e, 1, 1), offsets=off)
+    with pytest.raises(ValueError, match="65533 experts"):
+        ex.fp8_weight_grad(q.expand(4, 128), s.expand(4, 1),
+                           q.expand(8, 128), s.expand(8, 1), offsets=off)
 
 
 def _operands(rows=4, n=8, inner=200, experts=0):

@@ -889,6 +889,28 @@ def test_tiles_of_a_weight_gradient(at, m, n, out):
                            (a[:, part] @ b[:, part].t()).to(out)), e
 
 
+@pytest.mark.parametrize("rows", [3, 40])
+def test_as_many_experts_as_there_may_be(rows):
+    e, n, inner = 65533, 8, 128
+    gen = torch.Generator(device="cuda").manual_seed(rows)
+    a, qa, sa = whole_numbers(gen, rows, inner)
+    b, qb, _ = whole_numbers(gen, e, n, inner)
+    sb = torch.ones(e, 1, 1, device="cuda").to(E8)
+    off = torch.zeros(e + 1, dtype=torch.int32)
+    off[1000:] = 1
+    off[e] = rows
+    got = ex.fp8_matmul(qa, sa, qb, sb, dtype=torch.float32,
+                        offsets=off.cuda())
+    assert torch.equal(got[:1], a[:1] @ b[999].t())
+    assert torch.equal(got[1:], a[1:] @ b[e - 1].t())
+    x, qx, sx = whole_numbers(gen, n, rows)
+    got = ex.fp8_weight_grad(qx, sx, qx, sx, offsets=off.cuda())
+    ref = torch.zeros(e, n, n, device="cuda")
+    ref[999] = x[:, :1] @ x[:, :1].t()
+    ref[e - 1] = x[:, 1:] @ x[:, 1:].t()
+    assert torch.equal(got, ref)
+
+
 def test_single_rows_of_any_stride():
     gen = torch.Generator().manual_seed(6)
     a, sa = operand((1, 512), (1, 4), gen)
