@@ -442,9 +442,12 @@ PYBIND11_MODULE(_operators, m) {
   m.doc() = "The tensors' side of gloo_amd.experts";
 
   m.def("set_launchers", [](const py::capsule& c) {
-    launchers =
-        *static_cast<hip::ExpertLaunchers*>(PyCapsule_GetPointer(
-            c.ptr(), hip::kExpertLaunchers));
+    const auto* given = static_cast<hip::ExpertLaunchers*>(
+        PyCapsule_GetPointer(c.ptr(), hip::kExpertLaunchers));
+    if (given == nullptr) {
+      throw py::error_already_set();
+    }
+    launchers = *given;
   });
 
   m.def(
