@@ -69,7 +69,8 @@ struct Fp8ProductArgs {
   DType dtype = DType::BF16; // of out: F32, F16 or BF16
 };
 // out[r] = b[e] a[r] for the rows of each expert; zeros for rows before the
-// first expert's and behind the last one's.
+// first expert's and behind the last one's. Sums are fp32's; for BF16 groups
+// of eight products lose their bits below 2^-13 of the largest first.
 void launchFp8Matmul(
     const Fp8ProductArgs& args,
     int device,

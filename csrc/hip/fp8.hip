@@ -634,12 +634,18 @@ __device__ inline void swapQuarters(uint32_t& a, uint32_t& b) {
 // Native: v_mfma_scale_f32_32x32x64_f8f6f4 takes bytes and scales as they
 // are, at twice the rate of 16-bit operands. It adds groups of eight products
 // whose bits below 2^-13 of the group's largest one are cut (measured with
-// single products of known size; the groups' sums are added in full fp32).
-// That is finer than a result of 16 bits by itself, so those take it.
-// Exact: fp32 results show the cut. The bytes become bf16 with the scale
-// applied (no rounding: e4m3 has four bits, bf16 eight, and their exponents
-// are fp32's; below 2^-126 bits are lost) and the bf16 instruction, whose
-// groups are added with 24 bits, multiplies those.
+// single products of known size; the groups' sums are added in full fp32):
+// seven of a group lose up to 7 * 2^-13 < 2^-10 of the largest. bf16 results
+// take it: that is a quarter of half their step, 2^-8 (with random operands it
+// is 1.5e-5 of the result's norm). fp16 results, half a step of which is 2^-11,
+// do not, at the cost of time: 4095 x 8192 x 4096 242 us, bf16 117.
+// Exact: fp32 and fp16 results show the cut. The bytes become bf16 with the
+// scale applied (no rounding: e4m3 has four bits, bf16 eight, and their
+// exponents are fp32's; below 2^-126 bits are lost) and the bf16 instruction,
+// whose groups are added with 24 bits, multiplies those.
+template <typename O>
+constexpr bool kExactSums = !std::is_same<O, __hip_bfloat16>::value;
+
 template <bool kExact>
 struct Fragment;
 
@@ -889,7 +895,7 @@ __device__ inline void arrived() {
 template <typename O, bool kWeightGrad, int TM, int TN, int WM, int WN, int S>
 struct Product {
   using T = Tile<TM, TN, WM, WN>;
-  static constexpr bool kExact = std::is_same<O, float>::value;
+  static constexpr bool kExact = kExactSums<O>;
   const Job& job;
   int64_t n;
   int lane;
@@ -921,6 +927,7 @@ struct Product {
   __device__ void write(O* __restrict__ out, bool stream) const {
     constexpr int kEach = 16 / sizeof(O); // a lane's columns
     constexpr int kParts = 8 / kEach; // of 32 columns
+    constexpr bool kFull = sizeof(O) == 4;
     const bool whole = n % kEach == 0;
     const int quarter = lane / 16;
 #pragma unroll
@@ -930,7 +937,7 @@ struct Product {
 #pragma unroll
         for (int c = 0; c < kParts; c++) {
           uint32_t v[2][4]; // rows 0 to 15, and 16 to 31
-          if constexpr (kExact) {
+          if constexpr (kFull) {
 #pragma unroll
             for (int r = 0; r < 4; r++) {
               v[0][r] = __float_as_uint(acc[i][j][c * 8 + r]);
@@ -955,7 +962,7 @@ struct Product {
             }
           }
           const int64_t col = job.n0 + waveN + i * 32 +
-              (kExact ? c * 16 + quarter * 4
+              (kFull ? c * 16 + quarter * 4
                       : quarter % 2 * 16 + quarter / 2 * 8);
 #pragma unroll
           for (int r = 0; r < 2; r++) {
@@ -1418,7 +1425,7 @@ template <typename O, int MT, int kWaves>
 __global__ __launch_bounds__(kWaves * kWave) void fewRowsKernel(
     ProductShape p,
     O* __restrict__ out) {
-  constexpr bool kExact = std::is_same<O, float>::value;
+  constexpr bool kExact = kExactSums<O>;
   constexpr int kAhead = MT == 1 ? 4 : 2; // blocks on their way
   __shared__ float4 partial[kWaves][MT][kWave];
   const int lane = threadIdx.x % kWave;
@@ -1616,7 +1623,7 @@ weightGradKernel(ProductShape p, O* __restrict__ out) {
 // weight gradient of 16384 rows, 2048 x 2048 and 1024 x 1024:
 //                          139        92.8     108.9    136.1
 //                          136        86.9      57.1     39.2
-// Wider ones still, for 16-bit results: 256 x 256 424 for the first of these,
+// Wider ones still, for bf16 results: 256 x 256 424 for the first of these,
 // for 32 experts 16384 x 4096 x 4096 318 against 356 us with 128 x 256, if
 // experts have rows for them (each has a part of a tile that is empty).
 using WideTile = Tile<2, 4, 4, 2>;
@@ -1632,7 +1639,7 @@ constexpr int64_t kEnough = 192;
 // 2048 (about eight steps): 367 us against 414 with the large tile for fp32
 // results, 250 / 290 for bf16; 4 experts, some 32 steps, are even.
 constexpr int kShort = 32;
-// So are products with fp32 results and a short inner dimension: 8192 x 4096 x
+// So are products with fp32 or fp16 results and a short inner dimension: 8192 x 4096 x
 // 512 48 us against 50, 8741 x 4096 x 512 of 8 experts 62 / 72, 16384 x 2048 x
 // 1024 of 16 84 / 95, 8192 x 8192 x 2048 244 / 255; from there on even.
 constexpr int kShortInner = 16;
@@ -1648,7 +1655,7 @@ int64_t tilesOf(T, const ProductShape& p, bool grouped) {
 // How many times 16 rows fewRowsKernel takes at a time, 0 where tiles are
 // better. Measured by 8192 x 4096, this kernel and tiles in us, for bf16
 // results: 1 row 7 / 10.4, 4 rows 8.2 / 10.2, 16 rows 10.8 / 10.6; for fp32
-// ones, whose tiles take longer: 16 rows 13.6 / 15.2, 32 rows 18.1 / 15.4 (by
+// (and fp16) ones, whose tiles take longer: 16 rows 13.6 / 15.2, 32 rows 18.1 / 15.4 (by
 // 4096 x 4096 10.4 / 15.5). 8 rows for 8 of 16 experts of 1024 x 4096 8.5 /
 // 11.9, of 32 of 4096 x 2048 14.9 / 13.8, 16 rows of 16 experts 19.6 / 13.4;
 // fp32 4 rows 8.2 / 16.5 and 11.3 / 10.9, 8 rows 12.6 / 16.5 and 18.8 / 15.7.
@@ -1846,8 +1853,7 @@ void launchFp8Matmul(
       return tilesOf(tile, p, a.offsets != nullptr) *
           ((p.n + decltype(tile)::kN - 1) / decltype(tile)::kN);
     };
-    const int few = fewRows(
-        p, a.offsets != nullptr, std::is_same<O, float>::value);
+    const int few = fewRows(p, a.offsets != nullptr, kExactSums<O>);
     if (few != 0) {
       const auto goFew = [&](auto rows, auto waves) {
         constexpr int kRows = decltype(rows)::value;
@@ -1867,7 +1873,7 @@ void launchFp8Matmul(
           goFew(rows, std::integral_constant<int, 4>{});
         }
       };
-      if constexpr (std::is_same<O, float>::value) {
+      if constexpr (kExactSums<O>) {
         if (few == 2) {
           goWaves(std::integral_constant<int, 2>{});
           return;
@@ -1876,13 +1882,13 @@ void launchFp8Matmul(
       goWaves(std::integral_constant<int, 1>{});
       return;
     }
-    if constexpr (!std::is_same<O, float>::value) {
+    if constexpr (!kExactSums<O>) {
       if (tiles(WideTile{}) >= kEnough && p.m >= kWideRows * p.experts) {
         go(matmulKernel<O, 2, 4, 4, 2, kWideStages>, WideTile{});
         return;
       }
     }
-    if constexpr (std::is_same<O, float>::value) {
+    if constexpr (kExactSums<O>) {
       if (tiles(LargeTile{}) >= kEnough && p.inner <= kShortInner * kQuant) {
         go(matmulKernel<O, 2, 2, 2, 2, 2>, SmallTile{});
         return;

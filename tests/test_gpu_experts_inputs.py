@@ -1,0 +1,108 @@
+"""Expert operators on inputs that are not plain tensors, and on values where
+sums and exponentials lose what matters.
+
+Tolerances count roundings, as in test_gpu_experts.py, and its tests' names
+and order hold here too: these run behind test_gpu.py."""
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from gloo_amd import experts as ex  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("no GPU", allow_module_level=True)
+
+F8, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+U = 2.0 ** -24  # half a step of fp32
+
+
+def nb(n):
+    return -(-n // 128)
+
+
+def same(got, want):
+    for a, b in zip(got, want):
+        assert torch.equal(a.float(), b.float())
+
+
+# ------------------------------------------------- sums of 16-bit results
+
+
+def off_by_one_large(rows, inner, gen):
+    """One value of 448 in each block of 128, small ones of one sign: what is
+    cut below the largest of a few products is missed in the sum."""
+    x = torch.full((rows, nb(inner) * 128), 0.0234375)
+    at = torch.randint(0, 128, (rows, nb(inner), 1), generator=gen)
+    x.view(rows, nb(inner), 128).scatter_(2, at, 448.0)
+    return x[:, :inner].contiguous()
+
+
+SHAPES = [(1, 64, 128), (7, 130, 200), (16, 100, 300), (31, 70, 512),
+          (40, 130, 128), (300, 516, 256), (1024, 1300, 384),
+          (2500, 2570, 656), (4200, 4100, 2176)]
+
+
+def check16(got, a, b, out):
+    ref, size = a.double() @ b.double().t(), a.abs().double() @ \
+        b.abs().double().t()
+    half = torch.finfo(out).eps / 2
+    # an addition in fp32 is off by a step at most; and fp16's smallest
+    most = half * ref.abs() + (1 + half) * 2 * U * a.shape[1] * size + \
+        2.0 ** -25
+    err = (got.double() - ref).abs()
+    assert (err <= most).all(), ((err - most).max().item(),
+                                 (err / size.clamp_min(1e-30)).max().item())
+
+
+@pytest.mark.parametrize("m,n,k", SHAPES)
+@pytest.mark.parametrize("kind", ["large", "random"])
+def test_float16_products_are_summed_in_32_bits(m, n, k, kind):
+    gen = torch.Generator().manual_seed(m + k)
+    if kind == "large":
+        a, b = off_by_one_large(m, k, gen), torch.ones(n, k)
+    else:
+        a = (torch.randn(m, k, generator=gen) * 4).to(F8).float()
+        b = (torch.randn(n, k, generator=gen) * 4).to(F8).float()
+    a, b = a.cuda(), b.cuda()
+    qa, qb = a.to(F8), b.to(F8)
+    sa = torch.full((m, nb(k)), 2.0 ** -6).to(E8).cuda()
+    one = torch.ones(nb(n), nb(k)).to(E8).cuda()
+    a = a * 2.0 ** -6
+    got = ex.fp8_matmul(qa, sa, qb, one, dtype=torch.float16)
+    check16(got, a, b, torch.float16)
+    off = torch.tensor([0, m // 3, m // 3, m], dtype=torch.int32).cuda()
+    got = ex.fp8_matmul(qa, sa, qb[None].expand(3, n, k),
+                        one[None].expand(3, nb(n), nb(k)), offsets=off,
+                        dtype=torch.float16)
+    check16(got, a, b, torch.float16)
+    ones = torch.ones(n, nb(k)).to(E8).cuda()
+    got = ex.fp8_weight_grad(qa, sa, qb, ones, dtype=torch.float16)
+    check16(got, a, b, torch.float16)
+    at = [0, k // 3, k // 3, k]
+    off = torch.tensor(at, dtype=torch.int32).cuda()
+    got = ex.fp8_weight_grad(qa, sa, qb, ones, offsets=off,
+                             dtype=torch.float16)
+    for e in range(3):
+        check16(got[e], a[:, at[e]:at[e + 1]], b[:, at[e]:at[e + 1]],
+                torch.float16)
+
+
+@pytest.mark.parametrize("out", [torch.float32, torch.float16,
+                                 torch.bfloat16])
+def test_products_repeat_themselves(out):
+    """The same inputs give the same bits, call by call."""
+    gen = torch.Generator().manual_seed(3)
+    for m, n, k in ((1, 512, 4096), (16, 512, 1024), (256, 1024, 2048),
+                    (4095, 1024, 512), (4096, 4096, 640)):
+        a, sa = ex.quantize_fp8(torch.randn(m, k, generator=gen).cuda())
+        b, sb = ex.quantize_fp8(
+            torch.randn(n, k, generator=gen).cuda(), tile=True)
+        x, sx = ex.quantize_fp8(torch.randn(n, k, generator=gen).cuda())
+        runs = [(ex.fp8_matmul(a, sa, b, sb, dtype=out),
+                 ex.fp8_weight_grad(a, sa, x, sx, dtype=out))
+                for _ in range(3)]
+        for run in runs[1:]:
+            same(run, runs[0])
