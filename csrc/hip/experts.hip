@@ -92,6 +92,10 @@ __device__ inline uint32_t orderOf(float v) {
   const uint32_t bits = __float_as_uint(v);
   return bits ^ (bits >> 31 ? 0xffffffffu : 0x80000000u);
 }
+__device__ inline float valueOf(uint32_t order) {
+  return __uint_as_float(
+      order ^ (order >> 31 ? 0x80000000u : 0xffffffffu));
+}
 
 // The largest of a wave's numbers, in every lane: six steps within the
 // vector unit, where shuffles would go through LDS.
@@ -223,7 +227,7 @@ __global__ __launch_bounds__(kBlock) void routeKernel(
   double top = 0;
   double inv = 1;
   double score[kPer];
-  if (!p.sigmoid) {
+  if (summed) {
     uint32_t most = 0;
 #pragma unroll
     for (int i = 0; i < kPer; i++) {
@@ -231,7 +235,7 @@ __global__ __launch_bounds__(kBlock) void routeKernel(
       most = most > o ? most : o;
     }
     most = waveMaxOrder(most);
-    top = __uint_as_float(most ^ (most >> 31 ? 0x80000000u : 0xffffffffu));
+    top = valueOf(most);
   }
   if (summed || all) {
     // the arguments of what cannot be chosen give 0 either way
@@ -396,6 +400,14 @@ __global__ __launch_bounds__(kBlock) void routeKernel(
       mine = expert;
       chosen = value;
     }
+  }
+  // Renormalised softmax weights are a softmax over the chosen logits: below
+  // their own largest one, since a bias may have kept the token's largest out,
+  // and all of them may lie so far below that one that their scores are 0.
+  // Without a bias the first one chosen is the largest.
+  if (!p.sigmoid && p.renormalize) {
+    top = kBias ? valueOf(waveMaxOrder(orderOf(chosen))) : laneOf(chosen, 0);
+    inv = 1;
   }
   double w = 0;
   if (mine >= 0) {

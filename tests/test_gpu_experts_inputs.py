@@ -28,6 +28,39 @@ def same(got, want):
         assert torch.equal(a.float(), b.float())
 
 
+# ----------------------------------------------------------- router's weights
+
+
+@pytest.mark.parametrize("gap", [0, 100, 700, 709, 720, 744, 746, 1000, 3e4])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("groups", [1, 4])
+def test_renormalised_weights_far_below_the_top(gap, dtype, groups):
+    """A bias keeps the largest logit out: weights are a softmax over the
+    chosen ones, however far below it they are, and sum up to the scale."""
+    gen = torch.Generator().manual_seed(int(gap))
+    t, e, k, scale = 9, 16, 3, 2.5
+    x = torch.randn(t, e, generator=gen).to(dtype).float() - gap
+    x[:, 0] = 2.0
+    x = x.to(dtype)
+    bias = torch.linspace(1, 4, e)
+    bias[0] = -9.0
+    xg = x.cuda().requires_grad_()
+    w, ids = ex.route(xg, k, bias=bias.cuda(), groups=groups,
+                      topk_groups=groups, scale=scale)
+    assert (ids > 0).all()
+    g = torch.randn(t, k, generator=gen)
+    dx, = torch.autograd.grad(w, xg, g.cuda())
+    y = x.double().requires_grad_()
+    ref = scale * torch.softmax(y.gather(1, ids.cpu().long()), 1)
+    want, = torch.autograd.grad(ref, y, g.double())
+    err = (w.detach().double().cpu() - ref.detach()).abs()
+    assert (err <= ref * (U + 2.0 ** -44)).all(), err.max()
+    half = torch.finfo(dtype).eps / 2
+    slack = g.abs().max().item() * scale * k * 2.0 ** -40
+    most = (want.abs() + slack) * (half + U) + slack
+    assert ((dx.double().cpu() - want).abs() <= most).all()
+
+
 # ------------------------------------------------- sums of 16-bit results
 
 
