@@ -48,8 +48,28 @@ hipStream_t toStream(int64_t s) {
   return reinterpret_cast<hipStream_t>(s);
 }
 
-Tensor adjacent(const Tensor& t) {
+// What a tensor's memory holds is its values: not those of a view with the
+// negative bit set (the imaginary part of a conjugate is one), and not a zero
+// that has no memory. Data pointers are taken behind torch's dispatcher, which
+// would see to both. Differentiable.
+Tensor plain(const Tensor& t) {
+  if (t.defined() && (t.is_neg() || t._is_zerotensor())) {
+    return t.is_neg() ? t.resolve_neg() : at::zeros(t.sizes(), t.options());
+  }
+  return t;
+}
+
+std::optional<Tensor> plain(const std::optional<Tensor>& t) {
+  return t.has_value() ? std::optional<Tensor>(plain(*t)) : t;
+}
+
+Tensor adjacent(const Tensor& given) {
+  const Tensor t = plain(given);
   return t.stride(-1) == 1 || t.size(-1) == 1 ? t : t.contiguous();
+}
+
+Tensor contiguous(const Tensor& t) {
+  return plain(t).contiguous();
 }
 
 bool differentiated(const Tensor& t) {
@@ -137,7 +157,7 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
     once();
     const auto saved = ctx->get_saved_variables();
     const Tensor x = adjacent(saved[0]);
-    const Tensor grad = grads[0].contiguous();
+    const Tensor grad = contiguous(grads[0]);
     const int64_t bits = ctx->saved_data["options"].toInt();
     RouteOptions o{};
     o.k = bits >> 2;
@@ -160,7 +180,7 @@ struct RouteNode : public torch::autograd::Function<RouteNode> {
 
 std::tuple<Tensor, Tensor, Tensor>
 plan(const Tensor& experts, int64_t numExperts, int64_t stream) {
-  const Tensor ids = experts.contiguous();
+  const Tensor ids = contiguous(experts);
   Tensor position = at::empty(ids.sizes(), ids.options());
   Tensor counts = at::empty({numExperts}, ids.options());
   Tensor offsets = at::empty({numExperts + 1}, ids.options());
@@ -306,8 +326,9 @@ Tensor fp8Scales(at::IntArrayRef shape, const Tensor& like) {
 }
 
 std::pair<Tensor, Tensor>
-packFp8(const Tensor& tokens, const Tensor& position, int64_t stream) {
+packFp8(const Tensor& tokens, const Tensor& positions, int64_t stream) {
   const Tensor x = adjacent(tokens);
+  const Tensor position = plain(positions);
   const int64_t n = position.numel();
   auto [q, pitch] = fp8Rows({n}, x.size(1), x);
   Tensor scales = fp8Scales({n, blocksOf(x.size(1))}, x);
@@ -321,7 +342,8 @@ packFp8(const Tensor& tokens, const Tensor& position, int64_t stream) {
 }
 
 std::pair<Tensor, Tensor>
-quantize(const Tensor& x, bool tile, int64_t stream) {
+quantize(const Tensor& given, bool tile, int64_t stream) {
+  const Tensor x = plain(given);
   const int64_t rows = x.size(-2);
   const int64_t cols = x.size(-1);
   const bool many = x.dim() == 3;
@@ -364,13 +386,14 @@ Tensor matmul(
     const Tensor& aScaleGiven,
     const Tensor& bGiven,
     const Tensor& bScaleGiven,
-    const std::optional<Tensor>& offsets,
+    const std::optional<Tensor>& offsetsGiven,
     at::ScalarType dtype,
     int64_t stream) {
+  const auto offsets = plain(offsetsGiven);
   const Tensor a = adjacent(aGiven);
   const Tensor b = adjacent(bGiven);
-  const Tensor aScale = aScaleGiven.contiguous();
-  const Tensor bScale = bScaleGiven.contiguous();
+  const Tensor aScale = contiguous(aScaleGiven);
+  const Tensor bScale = contiguous(bScaleGiven);
   Tensor out =
       at::empty({a.size(0), b.size(-2)}, a.options().dtype(dtype));
   if (a.size(0) == 0) {
@@ -402,13 +425,14 @@ Tensor weightGrad(
     const Tensor& dyScaleGiven,
     const Tensor& xGiven,
     const Tensor& xScaleGiven,
-    const std::optional<Tensor>& offsets,
+    const std::optional<Tensor>& offsetsGiven,
     at::ScalarType dtype,
     int64_t stream) {
+  const auto offsets = plain(offsetsGiven);
   const Tensor dy = adjacent(dyGiven);
   const Tensor x = adjacent(xGiven);
-  const Tensor dyScale = dyScaleGiven.contiguous();
-  const Tensor xScale = xScaleGiven.contiguous();
+  const Tensor dyScale = contiguous(dyScaleGiven);
+  const Tensor xScale = contiguous(xScaleGiven);
   hip::Fp8WeightGradArgs p;
   p.m = dy.size(0);
   p.n = x.size(0);
@@ -452,9 +476,11 @@ PYBIND11_MODULE(_operators, m) {
 
   m.def(
       "route",
-      [](const Tensor& logits, const std::optional<Tensor>& bias, int64_t k,
-         bool sigmoid, int64_t groups, int64_t topkGroups, bool top2,
+      [](const Tensor& given, const std::optional<Tensor>& biasGiven,
+         int64_t k, bool sigmoid, int64_t groups, int64_t topkGroups, bool top2,
          bool renormalize, double scale, int64_t stream) {
+        const Tensor logits = plain(given);
+        const auto bias = plain(biasGiven);
         const RouteOptions o{k,    sigmoid,     groups, topkGroups,
                              top2, renormalize, scale};
         const auto out = differentiated(logits)
@@ -466,7 +492,9 @@ PYBIND11_MODULE(_operators, m) {
 
   m.def(
       "pack",
-      [](const Tensor& x, const Tensor& position, int64_t stream) {
+      [](const Tensor& given, const Tensor& positionGiven, int64_t stream) {
+        const Tensor x = plain(given);
+        const Tensor position = plain(positionGiven);
         return differentiated(x) ? PackNode::apply(x, position, stream)
                                  : packForward(x, position, stream);
       },
@@ -474,8 +502,11 @@ PYBIND11_MODULE(_operators, m) {
 
   m.def(
       "combine",
-      [](const Tensor& rows, const Tensor& position,
-         const std::optional<Tensor>& weights, int64_t stream) {
+      [](const Tensor& given, const Tensor& positionGiven,
+         const std::optional<Tensor>& weightsGiven, int64_t stream) {
+        const Tensor rows = plain(given);
+        const Tensor position = plain(positionGiven);
+        const auto weights = plain(weightsGiven);
         return differentiated(rows) || differentiated(orNone(weights))
             ? CombineNode::apply(rows, position, weights, stream)
             : combineForward(rows, position, orNone(weights), stream);

@@ -376,7 +376,8 @@ def _alltoall(pg, rows, send, recv):
     out = rows.new_empty((sum(recv),) + rows.shape[1:])
     if pg.size() == 1:
         return out.copy_(rows)
-    pg.alltoall_base(out, rows.contiguous(), recv, send,
+    # by memory: a negative view's would be the values' opposite
+    pg.alltoall_base(out, rows.resolve_neg().contiguous(), recv, send,
                      dist.AllToAllOptions()).wait()
     return out
 

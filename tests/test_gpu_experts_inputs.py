@@ -28,6 +28,77 @@ def same(got, want):
         assert torch.equal(a.float(), b.float())
 
 
+# ------------------------------------------------------------ negative views
+
+
+def negative(gen, *shape):
+    """Views whose values are the negated ones of their memory, as the
+    imaginary part of a conjugate is: of stride 2, and adjacent."""
+    z = torch.randn(shape, generator=gen, dtype=torch.complex64).cuda()
+    views = [z.conj().imag, torch._neg_view(z.real.contiguous())]
+    assert all(v.is_neg() for v in views)
+    return views
+
+
+def small_plan(t, k, e, gen):
+    ids = torch.stack([torch.randperm(e, generator=gen)[:k]
+                       for _ in range(t)]).to(torch.int32)
+    return ex.plan(ids.cuda(), e)
+
+
+@pytest.mark.parametrize("width", [1, 7, 64, 256])
+def test_negative_views(width):
+    gen = torch.Generator().manual_seed(width)
+    t, k, e = 12, 2, 8
+    p = small_plan(t, k, e, gen)
+    for v in negative(gen, t, width):
+        r = v.resolve_neg()
+        same(ex.quantize_fp8(v), ex.quantize_fp8(r))
+        same(ex.quantize_fp8(v.t()), ex.quantize_fp8(r.t()))
+        same(ex.quantize_fp8(v, tile=True), ex.quantize_fp8(r, tile=True))
+        same(ex.quantize_fp8(v.view(3, 4, width), tile=True),
+             ex.quantize_fp8(r.view(3, 4, width), tile=True))
+        same(ex.pack_fp8(v, p), ex.pack_fp8(r, p))
+        same([ex.pack(v, p)], [ex.pack(r, p)])
+        same(ex.route(v, 1), ex.route(r, 1))
+        same(ex.route(r, 1, bias=v[0]), ex.route(r, 1, bias=r[0]))
+    for w in negative(gen, t, k):
+        rows = torch.randn(t * k, width, generator=gen).cuda()
+        same([ex.combine(rows, p, w)], [ex.combine(rows, p, w.resolve_neg())])
+    for rows in negative(gen, t * k, width):
+        same([ex.combine(rows, p)], [ex.combine(rows.resolve_neg(), p)])
+
+
+@pytest.mark.parametrize("width", [1, 64])
+def test_gradients_of_negative_views(width):
+    """As inputs, and as what the gradient of the outputs is."""
+    gen = torch.Generator().manual_seed(width)
+    t, k, e = 12, 2, 8
+    p = small_plan(t, k, e, gen)
+    x = torch.randn(t, width, generator=gen).cuda().requires_grad_()
+    rows = torch.randn(t * k, width, generator=gen).cuda().requires_grad_()
+    w = torch.rand(t, k, generator=gen).cuda().requires_grad_()
+    z = torch.randn(t, e, generator=gen).cuda().requires_grad_()
+    calls = [(lambda a: ex.pack(a, p), (x,), (t * k, width)),
+             (lambda a, b: ex.combine(a, p, b), (rows, w), (t, width)),
+             (lambda a: ex.combine(a, p), (rows,), (t, width)),
+             (lambda a: ex.route(a, k)[0], (z,), (t, k))]
+    for call, leaves, shape in calls:
+        for g in negative(gen, *shape):
+            got = torch.autograd.grad(call(*leaves), leaves, g)
+            want = torch.autograd.grad(call(*leaves), leaves, g.resolve_neg())
+            same(got, want)
+        g = torch.randn(shape, generator=gen).cuda()
+        for i, leaf in enumerate(leaves):
+            for v in negative(gen, *leaf.shape):
+                v = v.detach().requires_grad_()
+                r = v.detach().resolve_neg().requires_grad_()
+                got, want = (torch.autograd.grad(
+                    call(*leaves[:i], y, *leaves[i + 1:]), y, g)
+                    for y in (v, r))
+                same(got, want)
+
+
 # ----------------------------------------------------------- router's weights
 
 
