@@ -15,6 +15,7 @@
 #include <torch/csrc/utils/pybind.h>
 
 #include <optional>
+#include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
@@ -70,6 +71,21 @@ Tensor adjacent(const Tensor& given) {
 
 Tensor contiguous(const Tensor& t) {
   return plain(t).contiguous();
+}
+
+// Operators have no forward-mode gradient, and a dual tensor's tangent would be
+// lost without a word.
+void noTangent(const char* name, const std::optional<Tensor>& t) {
+  if (t.has_value() && t->defined() && t->_fw_grad(/*level=*/0).defined()) {
+    throw py::value_error(
+        std::string(name) +
+        " has no forward-mode gradient: detach() its inputs");
+  }
+}
+
+template <typename... Ts>
+void noTangents(const char* name, const Ts&... ts) {
+  (noTangent(name, ts), ...);
 }
 
 bool differentiated(const Tensor& t) {
@@ -327,6 +343,7 @@ Tensor fp8Scales(at::IntArrayRef shape, const Tensor& like) {
 
 std::pair<Tensor, Tensor>
 packFp8(const Tensor& tokens, const Tensor& positions, int64_t stream) {
+  noTangents("pack_fp8", tokens);
   const Tensor x = adjacent(tokens);
   const Tensor position = plain(positions);
   const int64_t n = position.numel();
@@ -343,6 +360,7 @@ packFp8(const Tensor& tokens, const Tensor& positions, int64_t stream) {
 
 std::pair<Tensor, Tensor>
 quantize(const Tensor& given, bool tile, int64_t stream) {
+  noTangents("quantize_fp8", given);
   const Tensor x = plain(given);
   const int64_t rows = x.size(-2);
   const int64_t cols = x.size(-1);
@@ -390,6 +408,7 @@ Tensor matmul(
     at::ScalarType dtype,
     int64_t stream) {
   const auto offsets = plain(offsetsGiven);
+  noTangents("fp8_matmul", aGiven, aScaleGiven, bGiven, bScaleGiven);
   const Tensor a = adjacent(aGiven);
   const Tensor b = adjacent(bGiven);
   const Tensor aScale = contiguous(aScaleGiven);
@@ -429,6 +448,8 @@ Tensor weightGrad(
     at::ScalarType dtype,
     int64_t stream) {
   const auto offsets = plain(offsetsGiven);
+  noTangents(
+      "fp8_weight_grad", dyGiven, dyScaleGiven, xGiven, xScaleGiven);
   const Tensor dy = adjacent(dyGiven);
   const Tensor x = adjacent(xGiven);
   const Tensor dyScale = contiguous(dyScaleGiven);
@@ -479,6 +500,7 @@ PYBIND11_MODULE(_operators, m) {
       [](const Tensor& given, const std::optional<Tensor>& biasGiven,
          int64_t k, bool sigmoid, int64_t groups, int64_t topkGroups, bool top2,
          bool renormalize, double scale, int64_t stream) {
+        noTangents("route", given);
         const Tensor logits = plain(given);
         const auto bias = plain(biasGiven);
         const RouteOptions o{k,    sigmoid,     groups, topkGroups,
@@ -493,6 +515,7 @@ PYBIND11_MODULE(_operators, m) {
   m.def(
       "pack",
       [](const Tensor& given, const Tensor& positionGiven, int64_t stream) {
+        noTangents("pack", given);
         const Tensor x = plain(given);
         const Tensor position = plain(positionGiven);
         return differentiated(x) ? PackNode::apply(x, position, stream)
@@ -504,6 +527,7 @@ PYBIND11_MODULE(_operators, m) {
       "combine",
       [](const Tensor& given, const Tensor& positionGiven,
          const std::optional<Tensor>& weightsGiven, int64_t stream) {
+        noTangents("combine", given, weightsGiven);
         const Tensor rows = plain(given);
         const Tensor position = plain(positionGiven);
         const auto weights = plain(weightsGiven);

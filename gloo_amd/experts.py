@@ -14,7 +14,8 @@ run asynchronously on the current stream of their tensors' device, allocate
 with torch's allocator and may be captured into a graph (a backward pass only
 while no autograd graph of the same leaves from outside the capture is alive,
 as torch has it). Tensors have to be on a GPU; wrong arguments raise
-ValueError before anything is launched.
+ValueError before anything is launched, and so do inputs with a forward-mode
+gradient, which no operator has.
 
 8-bit values are torch.float8_e4m3fn. Their scales are powers of two
 (torch.float8_e8m0fnu): the least that brings a block's largest value to 448

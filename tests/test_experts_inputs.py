@@ -3,6 +3,8 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
+import torch.autograd.forward_ad as fw  # noqa: E402
+
 from gloo_amd import experts as ex  # noqa: E402
 
 
@@ -29,3 +31,36 @@ def test_negative_rows_between_ranks():
         return True
 
     spawn_pg(2, fn)
+
+
+def test_forward_mode_is_refused():
+    """Below the check of the device, on batches without tokens: an input's
+    tangent would be lost."""
+    ops = ex._ops
+    ids = torch.zeros(0, 2, dtype=torch.int32)
+    q = torch.zeros(0, 128).to(torch.float8_e4m3fn)
+    s = torch.zeros(0, 1).to(torch.float8_e8m0fnu)
+    b, bs = torch.zeros(4, 128).to(q.dtype), torch.ones(1, 1).to(s.dtype)
+    with fw.dual_level():
+        for grad in (False, True):
+            def dual(v):
+                return fw.make_dual(v.clone().requires_grad_(grad),
+                                    torch.ones_like(v))
+
+            x = torch.zeros(0, 8)
+            calls = [
+                lambda: ops.route(dual(x), None, 2, False, 1, 1, False, True,
+                                  1.0, 0),
+                lambda: ops.pack(dual(x), ids, 0),
+                lambda: ops.combine(dual(x), ids, None, 0),
+                lambda: ops.combine(x, ids, dual(torch.zeros(0, 2)), 0),
+                lambda: ops.pack_fp8(dual(x), ids, 0),
+                lambda: ops.quantize_fp8(dual(x), False, 0),
+                lambda: ops.fp8_matmul(dual(q), s, b, bs, None,
+                                       torch.float32, 0),
+                lambda: ops.fp8_matmul(q, s, dual(b), bs, None,
+                                       torch.float32, 0)]
+            for call in calls:
+                with pytest.raises(ValueError, match="forward-mode"):
+                    call()
+        ops.pack(dual(x).detach(), ids, 0)

@@ -3,10 +3,11 @@ sums and exponentials lose what matters.
 
 Tolerances count roundings, as in test_gpu_experts.py, and its tests' names
 and order hold here too: these run behind test_gpu.py."""
-
 import pytest
 
 torch = pytest.importorskip("torch")
+
+import torch.autograd.forward_ad as fw  # noqa: E402
 
 from gloo_amd import experts as ex  # noqa: E402
 
@@ -97,6 +98,43 @@ def test_gradients_of_negative_views(width):
                     call(*leaves[:i], y, *leaves[i + 1:]), y, g)
                     for y in (v, r))
                 same(got, want)
+
+
+# ------------------------------------------------------- forward-mode inputs
+
+
+def test_forward_mode_is_refused():
+    """A dual tensor's tangent would be lost without a word."""
+    gen = torch.Generator().manual_seed(1)
+    t, k, e = 12, 2, 8
+    p = small_plan(t, k, e, gen)
+    x = torch.randn(t, 64, generator=gen).cuda()
+    rows = torch.randn(t * k, 64, generator=gen).cuda()
+    w = torch.rand(t, k, generator=gen).cuda()
+    q, s = ex.quantize_fp8(x)
+    b, bs = ex.quantize_fp8(x, tile=True)
+    with fw.dual_level():
+        for grad in (False, True):
+            def dual(v):
+                return fw.make_dual(v.clone().requires_grad_(grad),
+                                    torch.ones_like(v))
+
+            calls = [lambda: ex.route(dual(x), 2),
+                     lambda: ex.pack(dual(x), p),
+                     lambda: ex.pack_fp8(dual(x), p),
+                     lambda: ex.combine(dual(rows), p),
+                     lambda: ex.combine(dual(rows), p, w),
+                     lambda: ex.combine(rows, p, dual(w)),
+                     lambda: ex.quantize_fp8(dual(x)),
+                     lambda: ex.quantize_fp8(dual(x), tile=True),
+                     lambda: ex.fp8_matmul(dual(q), s, b, bs),
+                     lambda: ex.fp8_matmul(q, s, dual(b), bs),
+                     lambda: ex.fp8_weight_grad(dual(q), s, q, s),
+                     lambda: ex.fp8_weight_grad(q, s, dual(q), s)]
+            for call in calls:
+                with pytest.raises(ValueError, match="gradient"):
+                    call()
+        ex.pack(dual(x).detach(), p)  # its value alone
 
 
 # ----------------------------------------------------------- router's weights
