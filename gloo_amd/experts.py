@@ -307,8 +307,9 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
     b_scale have a leading dimension for experts, and rows offsets[e] to
     offsets[e + 1] are multiplied by b[e]; rows before the first expert's (some
     of a plan's experts will do) and behind the last one's are zeros. The data
-    gradient is the same product with the weights' transposed copy;
-    `fp8_weight_grad` is the other one."""
+    gradient is the same product with the weights' transposed copy, and
+    `fp8_weight_grad` is the other one: operands that want a gradient are
+    refused."""
     if not isinstance(a, torch.Tensor) or a.dim() != 2:
         raise ValueError("a: a tensor of 2 dimensions is needed")
     if (not isinstance(b, torch.Tensor)
@@ -329,6 +330,7 @@ def fp8_matmul(a, a_scale, b, b_scale, offsets=None, dtype=torch.bfloat16):
     _fp8_operand(b, b_scale, "b", b.dim(),
                  tuple(b.shape[:-2]) + (_blocks(n), _blocks(inner)), a)
     _offsets(offsets, experts, a)
+    _no_gradient("fp8_matmul", a, a_scale, b, b_scale)
     _gpu(a, "fp8_matmul")
     return _ops.fp8_matmul(a, a_scale, b, b_scale, offsets, dtype,
                            _stream(a))
@@ -344,7 +346,8 @@ def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
     `dtype`, added up and rounded as `fp8_matmul` does it. With `offsets` (int32
     [experts + 1]) rows offsets[e] to offsets[e + 1] are expert e's, and the
     result is [experts, m, n], zeros for an expert without rows. Experts may
-    begin anywhere: two of them can share a block and its scale."""
+    begin anywhere: two of them can share a block and its scale. It has no
+    gradient."""
     if (not isinstance(dy, torch.Tensor) or dy.dim() != 2 or not
             isinstance(x, torch.Tensor) or x.dim() != 2):
         raise ValueError("dy, x: tensors of 2 dimensions are needed")
@@ -364,6 +367,7 @@ def fp8_weight_grad(dy, dy_scale, x, x_scale, offsets=None,
         raise ValueError(f"offsets: [experts + 1] is needed, for 1 to "
                          f"{_FP8_EXPERTS} experts")
     _offsets(offsets, 0 if offsets is None else offsets.shape[0] - 1, dy)
+    _no_gradient("fp8_weight_grad", dy, dy_scale, x, x_scale)
     _gpu(dy, "fp8_weight_grad")
     return _ops.fp8_weight_grad(dy, dy_scale, x, x_scale, offsets, dtype,
                                 _stream(dy))

@@ -64,3 +64,20 @@ def test_forward_mode_is_refused():
                 with pytest.raises(ValueError, match="forward-mode"):
                     call()
         ops.pack(dual(x).detach(), ids, 0)
+
+
+def test_products_refuse_operands_with_a_gradient():
+    """x.to(float8) is differentiable in torch, products of it are not."""
+    x = torch.zeros(4, 128, requires_grad=True)
+    q, s = x.to(torch.float8_e4m3fn), torch.ones(4, 1).to(
+        torch.float8_e8m0fnu)
+    w, ws = q.detach(), torch.ones(1, 1).to(s.dtype)
+    assert q.requires_grad
+    for call in (lambda: ex.fp8_matmul(q, s, w, ws),
+                 lambda: ex.fp8_matmul(w, s, q, ws),
+                 lambda: ex.fp8_weight_grad(q, s, w, s),
+                 lambda: ex.fp8_weight_grad(w, s, q, s)):
+        with pytest.raises(ValueError, match="no gradient"):
+            call()
+        with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):
+            call()
