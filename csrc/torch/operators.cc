@@ -14,12 +14,14 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <exception>
 #include <optional>
 #include <string>
 #include <tuple>
 #include <utility>
 #include <vector>
 
+#include "common/error.h"
 #include "hip/expert_launchers.h"
 
 namespace py = pybind11;
@@ -485,6 +487,15 @@ PYBIND11_MODULE(_operators, m) {
   using namespace glooamd;
   using Unlocked = py::call_guard<py::gil_scoped_release>;
   m.doc() = "The tensors' side of gloo_amd.experts";
+
+  // What a launch refuses (a grid that it cannot hold) is a wrong argument.
+  py::register_local_exception_translator([](std::exception_ptr p) {
+    try {
+      std::rethrow_exception(p);
+    } catch (const EnforceNotMet& e) {
+      PyErr_SetString(PyExc_ValueError, e.what());
+    }
+  });
 
   m.def("set_launchers", [](const py::capsule& c) {
     const auto* given = static_cast<hip::ExpertLaunchers*>(

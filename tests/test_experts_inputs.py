@@ -81,3 +81,11 @@ def test_products_refuse_operands_with_a_gradient():
             call()
         with torch.no_grad(), pytest.raises(ValueError, match="on a GPU"):
             call()
+
+
+def test_what_a_launch_refuses_is_a_wrong_argument():
+    """Launches check for themselves, before they touch a device."""
+    for k, groups in ((9, 1), (2, 3)):
+        with pytest.raises(ValueError):
+            ex._ops.route(torch.zeros(0, 8), None, k, False, groups, 1, False,
+                          True, 1.0, 0)

@@ -248,3 +248,19 @@ def test_products_repeat_themselves(out):
                 for _ in range(3)]
         for run in runs[1:]:
             same(run, runs[0])
+
+
+# ------------------------------------------------- refusals by the launches
+
+
+def test_launches_that_are_too_large_are_wrong_arguments():
+    one = torch.ones(1, device="cuda")
+    with pytest.raises(ValueError):
+        ex.quantize_fp8(one.expand(2 ** 24, 1, 1), tile=True)
+    e, n = 65533, 257 * 128
+    q, s = one.to(F8), one.to(E8)
+    off = torch.zeros(e + 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError):
+        ex.fp8_weight_grad(q.expand(1, 8), s.expand(1, 1), q.expand(n, 8),
+                           s.expand(n, 1), offsets=off,
+                           dtype=torch.bfloat16)
