@@ -288,7 +288,9 @@ struct CombineNode : public torch::autograd::Function<CombineNode> {
       const std::optional<Tensor>& given,
       int64_t stream) {
     const Tensor weights = orNone(given);
-    ctx->save_for_backward({rows, position, weights});
+    // Without weights the gradient needs no rows: they are free to change.
+    ctx->save_for_backward(
+        {weights.defined() ? rows : Tensor(), position, weights});
     ctx->saved_data["stream"] = stream;
     return combineForward(rows, position, weights, stream);
   }

@@ -250,6 +250,23 @@ def test_products_repeat_themselves(out):
             same(run, runs[0])
 
 
+# ---------------------------------------------------------------- what is kept
+
+
+def test_sums_without_weights_keep_no_rows():
+    """Their gradient does not need them: they may change, and are free."""
+    gen = torch.Generator().manual_seed(4)
+    p = small_plan(12, 2, 8, gen)
+    leaf = torch.randn(24, 64, generator=gen).cuda().requires_grad_()
+    g = torch.randn(12, 64, generator=gen).cuda()
+    want, = torch.autograd.grad(ex.combine(leaf * 1, p), leaf, g)
+    rows = leaf * 1
+    out = ex.combine(rows, p)
+    rows.zero_()
+    got, = torch.autograd.grad(out, leaf, g)
+    assert torch.equal(got, want)
+
+
 # ------------------------------------------------- refusals by the launches
 
 
