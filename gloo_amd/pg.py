@@ -357,8 +357,9 @@ class ProcessGroupGlooAmd(dist.ProcessGroup):
                 ga.alltoall(self._ctx, h_out.data_ptr(), h_in.data_ptr(),
                             per, _gdtype(inp), tag=tag)
             else:
-                # of the shape and not of the count: a rank may have no rows
-                row = inp.shape[1:].numel()
+                # of the shape and not of the count: a rank may have no
+                # rows, and an input without any may tell no shape either
+                row = (inp if inp.numel() else out).shape[1:].numel()
                 in_counts = [int(s) * row for s in input_split_sizes]
                 out_counts = [int(s) * row for s in output_split_sizes]
                 ga.alltoallv(self._ctx, h_out.data_ptr(), h_in.data_ptr(),

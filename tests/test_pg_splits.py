@@ -29,3 +29,25 @@ def test_alltoall_splits_without_rows():
     for counts in ([[0, 0], [3, 2]], [[0, 3], [0, 2]], [[0, 0], [0, 0]]):
         for shape in ((), (5,)):
             spawn_pg(2, lambda pg, r, n: _exchange(pg, r, n, counts, shape))
+
+
+def test_alltoall_splits_of_plainly_empty_tensors():
+    """A rank without rows need not know their shape."""
+    counts = [[0, 0], [3, 2]]
+
+    def fn(pg, rank, size):
+        outs = [counts[s][rank] for s in range(size)]
+        inp = (torch.empty(0) if rank == 0 else
+               torch.arange(25.0).view(5, 5))
+        out = torch.full((sum(outs), 5), -1.0)
+        pg.alltoall_base(out, inp, outs, counts[rank]).wait()
+        at = slice(0, 3) if rank == 0 else slice(3, 5)
+        assert torch.equal(out, torch.arange(25.0).view(5, 5)[at])
+        # and the way back: the other rank's output is empty
+        back = torch.empty(0) if rank == 0 else torch.full((5, 5), -1.0)
+        pg.alltoall_base(back, out, counts[rank], outs).wait()
+        if rank == 1:
+            assert torch.equal(back, torch.arange(25.0).view(5, 5))
+        return True
+
+    spawn_pg(2, fn)
