@@ -5,6 +5,8 @@ Tolerances count roundings, as in test_gpu_experts.py, and its tests' names
 and order hold here too: these run behind test_gpu.py."""
 import pytest
 
+import gloo_amd as ga
+
 torch = pytest.importorskip("torch")
 
 import torch.autograd.forward_ad as fw  # noqa: E402
@@ -281,3 +283,43 @@ def test_launches_that_are_too_large_are_wrong_arguments():
         ex.fp8_weight_grad(q.expand(1, 8), s.expand(1, 1), q.expand(n, 8),
                            s.expand(n, 1), offsets=off,
                            dtype=torch.bfloat16)
+
+
+def test_wrong_offsets_leave_what_is_around_the_result():
+    """Offsets are read on the device. Wrong ones write nothing before or
+    behind the result, which lies in the middle of a larger buffer here."""
+    gen = torch.Generator().manual_seed(2)
+    c = ga._C
+    kinds = [(ga.DType.f32, torch.float32), (ga.DType.bf16, torch.bfloat16),
+             (ga.DType.f16, torch.float16)]
+    for rows in (3, 20, 700):
+        e, n, k, margin = 3, 72, 256, 4096
+        a, sa = ex.quantize_fp8(torch.randn(rows, k, generator=gen).cuda())
+        b, sb = ex.quantize_fp8(
+            torch.randn(e, n, k, generator=gen).cuda(), tile=True)
+        x, sx = ex.quantize_fp8(torch.randn(n, rows, generator=gen).cuda())
+        for at in ([-5, 3, 2 ** 31 - 1, 2 ** 30], [rows, 4, 2, 0],
+                   [-2 ** 31, -1, -1, 99], [0, rows, 0, rows],
+                   [2 ** 31 - 1] * 4):
+            off = torch.tensor(at, dtype=torch.int32).cuda()
+            for gdt, tdt in kinds:
+                for grad in (False, True):
+                    size = e * n * n if grad else rows * n
+                    room = torch.full((size + 2 * margin,), 7.0, dtype=tdt,
+                                      device="cuda")
+                    out = room[margin:margin + size]
+                    if grad:
+                        c.hip_fp8_weight_grad(
+                            x.data_ptr(), x.stride(0), sx.data_ptr(),
+                            x.data_ptr(), x.stride(0), sx.data_ptr(),
+                            off.data_ptr(), n, n, rows, e, out.data_ptr(),
+                            gdt, 0, 0)
+                    else:
+                        c.hip_fp8_matmul(
+                            a.data_ptr(), a.stride(0), sa.data_ptr(),
+                            b.data_ptr(), b.stride(1), b.stride(0),
+                            sb.data_ptr(), off.data_ptr(), rows, n, k, e,
+                            out.data_ptr(), gdt, 0, 0)
+                    torch.cuda.synchronize()
+                    assert (room[:margin] == 7).all()
+                    assert (room[margin + size:] == 7).all()
