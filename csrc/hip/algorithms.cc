@@ -1,6 +1,5 @@
 #include "hip/algorithms.h"
 
-#include <atomic>
 #include <chrono>
 #include <thread>
 
@@ -38,34 +37,7 @@ void watchdogWait(
   auto deadline = std::chrono::steady_clock::now() + timeout;
   while (!ev.query()) {
     if (timeout.count() > 0 && std::chrono::steady_clock::now() > deadline) {
-      std::string flags;
-      if (getEnvFlag("GLOO_AMD_FLAG_DEBUG")) {
-        uint64_t vals[16] = {0};
-        (void)hipMemcpy(vals, mesh.flag(0), sizeof(vals),
-                        hipMemcpyDeviceToHost);
-        for (int i = 0; i < 16; i++) {
-          flags += " " + std::to_string(vals[i]);
-        }
-      }
-      mesh.poisonFlags();
-      // Bounded drain: a wedged hardware queue can make
-      // hipDeviceSynchronize hang forever; give it a few seconds on a
-      // helper thread, then fail fast (a leaked sync thread on a
-      // broken device is acceptable in the fail-fast model — the
-      // throw is what keeps the job from hanging).
-      {
-        auto done = std::make_shared<std::atomic<bool>>(false);
-        std::thread([done] {
-          (void)hipDeviceSynchronize();
-          done->store(true);
-        }).detach();
-        const auto dl =
-            std::chrono::steady_clock::now() + std::chrono::seconds(8);
-        while (!done->load() && std::chrono::steady_clock::now() < dl) {
-          std::this_thread::sleep_for(std::chrono::milliseconds(10));
-        }
-      }
-      GA_THROW_IO("hip collective timed out in ", what, " flags:", flags);
+      mesh.fail(what);
     }
     std::this_thread::yield();
   }
@@ -410,7 +382,7 @@ int HipAllreduceRing::enqueueRing(
       const uint64_t prevAck =
           (k >= 2) ? seqOf(k - 2) : lastAckPerRing_[j][par];
       if (prevAck > 0) {
-        launchWaitFlagGte(mesh_->flag(fACK_[j] + par), prevAck, ksm);
+        mesh_->waitFlag(fACK_[j] + par, prevAck, ksm);
       }
     }
     if (k >= S) {
@@ -434,7 +406,7 @@ int HipAllreduceRing::enqueueRing(
     } else {
       launchWriteFlag(mesh_->peerFlag(right, fDATA_[j] + par), seqOf(k),
                       ksm);
-      launchWaitFlagGte(mesh_->flag(fDATA_[j] + par), seqOf(k), csm);
+      mesh_->waitFlag(fDATA_[j] + par, seqOf(k), csm);
     }
     if (st.recv.len > 0) {
       if (st.reduceStep) {
@@ -502,7 +474,9 @@ void HipAllreduceRing::runDevice(
   // first run of a shape goes eager (exact cross-run gates) and capture
   // happens from the second run on.
   GraphKey key{buf, n, static_cast<int>(dt), static_cast<int>(op)};
-  if (graphsEnabled() && !graphBroken_ && lastKey_ == key) {
+  // (A graph's waits are the device's, so ranks that share one go without.)
+  if (graphsEnabled() && !graphBroken_ && !mesh_->sharesDevice() &&
+      lastKey_ == key) {
     if (runDeviceGraph(buf, n, es, dt, op)) {
       return;
     }
@@ -777,7 +751,7 @@ void HipAllreduceHalvingDoubling::run(
       const int par = c & 1;
       foldSeq_++;
       if (lastFold_[par] > 0) {
-        launchWaitFlagGte(mesh_->flag(fFACK_ + par), lastFold_[par], ksm);
+        mesh_->waitFlag(fFACK_ + par, lastFold_[par], ksm);
       }
       Seg ch = foldChunk(c);
       GA_HIP_CHECK(hipMemcpyAsync(
@@ -791,7 +765,7 @@ void HipAllreduceHalvingDoubling::run(
     }
     // Post-fold: partner writes the final result into our work region.
     postSeq_++;
-    launchWaitFlagGte(mesh_->flag(fPOST_), postSeq_, csm);
+    mesh_->waitFlag(fPOST_, postSeq_, csm);
     GA_HIP_CHECK(
         hipMemcpyAsync(buf, work, bytes, hipMemcpyDeviceToDevice, csm));
     launchWriteFlag(mesh_->peerFlag(partner, fPACK_), postSeq_, csm);
@@ -813,7 +787,7 @@ void HipAllreduceHalvingDoubling::run(
     for (int c = 0; c < foldNc; c++) {
       const int par = c & 1;
       foldSeq_++;
-      launchWaitFlagGte(mesh_->flag(fFOLD_ + par), foldSeq_, csm);
+      mesh_->waitFlag(fFOLD_ + par, foldSeq_, csm);
       Seg ch = foldChunk(c);
       launchReduce2(
           work + ch.off * es,
@@ -868,8 +842,7 @@ void HipAllreduceHalvingDoubling::run(
       seq_++;
       const uint64_t dseq = seq_;
       if (lastAck_[t * 2 + par] > 0) {
-        launchWaitFlagGte(
-            mesh_->flag(fACK_ + t * 2 + par), lastAck_[t * 2 + par], ksm);
+        mesh_->waitFlag(fACK_ + t * 2 + par, lastAck_[t * 2 + par], ksm);
       }
       Seg gch = sched::chunkOfA(gv, c, nc, A);
       if (gch.len > 0) {
@@ -882,7 +855,7 @@ void HipAllreduceHalvingDoubling::run(
       }
       launchWriteFlag(mesh_->peerFlag(peer, fDATA_ + t * 2 + par), dseq, ksm);
 
-      launchWaitFlagGte(mesh_->flag(fDATA_ + t * 2 + par), dseq, csm);
+      mesh_->waitFlag(fDATA_ + t * 2 + par, dseq, csm);
       Seg kch = sched::chunkOfA(kp, c, nc, A);
       if (kch.len > 0) {
         launchReduce2(
@@ -910,7 +883,7 @@ void HipAllreduceHalvingDoubling::run(
     } else {
       // Halves received in step t+1 are part of cur now.
       if (lastAgd_[t + 1] > 0) {
-        launchWaitFlagGte(mesh_->flag(fAGD_ + t + 1), lastAgd_[t + 1], ksm);
+        mesh_->waitFlag(fAGD_ + t + 1, lastAgd_[t + 1], ksm);
       }
     }
     seq_++;
@@ -930,7 +903,7 @@ void HipAllreduceHalvingDoubling::run(
 
   // Final: wait all incoming allgather halves, stage out.
   for (int t = 0; t < T; t++) {
-    launchWaitFlagGte(mesh_->flag(fAGD_ + t), lastAgd_[t], csm);
+    mesh_->waitFlag(fAGD_ + t, lastAgd_[t], csm);
   }
   if (r < extras) {
     // Post-fold: push the final result into the extra rank's work
@@ -939,7 +912,7 @@ void HipAllreduceHalvingDoubling::run(
     postSeq_++;
     const int extra = r + pow2_;
     if (postSeq_ > 1) {
-      launchWaitFlagGte(mesh_->flag(fPACK_), postSeq_ - 1, csm);
+      mesh_->waitFlag(fPACK_, postSeq_ - 1, csm);
     }
     GA_HIP_CHECK(hipMemcpyAsync(
         mesh_->peerWork(extra), work, bytes, hipMemcpyDeviceToDevice, csm));
@@ -1024,7 +997,7 @@ void HipBroadcastOneToAll::run(
       auto& st = *fanout_[si++ % fanout_.size()];
       staged.streamWait(st.stream());
       if (seq_ > 1) {
-        launchWaitFlagGte(mesh_->flag(fBACK_ + i), seq_ - 1, st.stream());
+        mesh_->waitFlag(fBACK_ + i, seq_ - 1, st.stream());
       }
       GA_HIP_CHECK(hipMemcpyAsync(
           mesh_->peerWork(i),
@@ -1042,7 +1015,7 @@ void HipBroadcastOneToAll::run(
       st->synchronize();
     }
   } else {
-    launchWaitFlagGte(mesh_->flag(fBDATA_), seq_, cs_->stream());
+    mesh_->waitFlag(fBDATA_, seq_, cs_->stream());
     GA_HIP_CHECK(hipMemcpyAsync(
         buf, work, bytes, hipMemcpyDeviceToDevice, cs_->stream()));
     launchWriteFlag(mesh_->peerFlag(root_, fBACK_ + r), seq_, cs_->stream());
@@ -1200,7 +1173,7 @@ void HipAllreduceDirect::run(
     auto& st = *fanout_[(j - 1) % fanout_.size()];
     if (runSeq > 1) {
       // d finished its previous copy-out before we touch its memory.
-      launchWaitFlagGte(mesh_->flag(fDONE_ + d), runSeq - 1, st.stream());
+      mesh_->waitFlag(fDONE_ + d, runSeq - 1, st.stream());
     }
   }
   for (int c = 0; c < C; c++) {
@@ -1211,7 +1184,7 @@ void HipAllreduceDirect::run(
       auto& st = *fanout_[(j - 1) % fanout_.size()];
       const uint64_t gate = (c >= 2) ? cseq(c - 2) : lastAck_[d][par];
       if (gate > 0) {
-        launchWaitFlagGte(mesh_->flag(fACK_ + d), gate, st.stream());
+        mesh_->waitFlag(fACK_ + d, gate, st.stream());
       }
       const size_t len = chunkLen(d, c);
       if (len > 0) {
@@ -1227,7 +1200,7 @@ void HipAllreduceDirect::run(
     // fused reduction of chunk c of my block
     for (int src = 0; src < P; src++) {
       if (src != r) {
-        launchWaitFlagGte(mesh_->flag(fRS_ + src), cseq(c), cs_->stream());
+        mesh_->waitFlag(fRS_ + src, cseq(c), cs_->stream());
       }
     }
     const size_t rlen = chunkLen(r, c);
@@ -1271,7 +1244,7 @@ void HipAllreduceDirect::run(
   // --- collect, stage out, publish copy-out-done (cs) ---
   for (int src = 0; src < P; src++) {
     if (src != r) {
-      launchWaitFlagGte(mesh_->flag(fAG_ + src), cseq(C - 1),
+      mesh_->waitFlag(fAG_ + src, cseq(C - 1),
                         cs_->stream());
     }
   }
@@ -1426,7 +1399,7 @@ void HipAllgatherRing::run(
 
     const uint64_t prevAck = (k >= 2) ? seqOf(k - 2) : lastAck_[par];
     if (prevAck > 0) {
-      launchWaitFlagGte(mesh_->flag(fACK_ + par), prevAck, ksm);
+      mesh_->waitFlag(fACK_ + par, prevAck, ksm);
     }
     if (k >= S) {
       events_[(k - S) % pool]->streamWait(ksm);
@@ -1443,7 +1416,7 @@ void HipAllgatherRing::run(
     }
     launchWriteFlag(mesh_->peerFlag(right, fDATA_ + par), seqOf(k), ksm);
 
-    launchWaitFlagGte(mesh_->flag(fDATA_ + par), seqOf(k), csm);
+    mesh_->waitFlag(fDATA_ + par, seqOf(k), csm);
     if (send.len > 0) {
       GA_HIP_CHECK(hipMemcpyAsync(
           work + recvBlock * blockBytes + send.off * es,
@@ -1554,7 +1527,7 @@ void HipReduceScatterRing::run(
 
     const uint64_t prevAck = (k >= 2) ? seqOf(k - 2) : lastAck_[par];
     if (prevAck > 0) {
-      launchWaitFlagGte(mesh_->flag(fACK_ + par), prevAck, ksm);
+      mesh_->waitFlag(fACK_ + par, prevAck, ksm);
     }
     if (k >= S) {
       events_[(k - S) % pool]->streamWait(ksm);
@@ -1571,7 +1544,7 @@ void HipReduceScatterRing::run(
     }
     launchWriteFlag(mesh_->peerFlag(right, fDATA_ + par), seqOf(k), ksm);
 
-    launchWaitFlagGte(mesh_->flag(fDATA_ + par), seqOf(k), csm);
+    mesh_->waitFlag(fDATA_ + par, seqOf(k), csm);
     if (seg.len > 0) {
       launchReduce2(
           work + recvBlock * blockBytes + seg.off * es,
@@ -1670,7 +1643,7 @@ void HipAlltoall::run(
     auto& st = *fanout_[si++ % fanout_.size()];
     if (seq > 1) {
       // d must have copied out the previous run's block from its work.
-      launchWaitFlagGte(mesh_->flag(fACK_ + d), seq - 1, st.stream());
+      mesh_->waitFlag(fACK_ + d, seq - 1, st.stream());
     }
     if (blockBytes > 0) {
       GA_HIP_CHECK(hipMemcpyAsync(
@@ -1694,7 +1667,7 @@ void HipAlltoall::run(
     if (s == r) {
       continue;
     }
-    launchWaitFlagGte(mesh_->flag(fDATA_ + s), seq, cs_->stream());
+    mesh_->waitFlag(fDATA_ + s, seq, cs_->stream());
     GA_HIP_CHECK(hipMemcpyAsync(
         out + static_cast<size_t>(s) * blockBytes,
         work + static_cast<size_t>(s) * blockBytes,
@@ -1756,30 +1729,17 @@ void HipP2P::postSend(
   TraceRange tr("gloo_amd::hip_p2p_send");
   std::lock_guard<std::mutex> lock(mu_);
   GA_HIP_CHECK(hipSetDevice(device_));
-  const int r = ctx_->rank;
-  GA_ENFORCE(dst != r, "p2p send to self");
+  GA_ENFORCE(dst != ctx_->rank, "p2p send to self");
   gateStreams(*gateSendEv_, callerStream, {ss_->stream()});
-  const char* src = static_cast<const char*>(devPtr);
+  // Sends do not write through the pointer.
+  char* src = static_cast<char*>(const_cast<void*>(devPtr));
   const size_t nc = (bytes + chunkCap_ - 1) / chunkCap_;
   for (size_t c = 0; c < std::max<size_t>(nc, 1); c++) {
-    const uint64_t seq = ++sendChunkSeq_[dst];
-    const int par = static_cast<int>(seq & 1);
-    if (seq > 2) {
-      // Same-parity slot reuse: dst consumed chunk seq-2.
-      launchWaitFlagGte(mesh_->flag(fACK_ + dst), seq - 2, ss_->stream());
-    }
     const size_t off = c * chunkCap_;
     const size_t len = std::min(chunkCap_, bytes - std::min(bytes, off));
-    if (len > 0) {
-      GA_HIP_CHECK(hipMemcpyAsync(
-          slotOf(mesh_->peerInbox(dst, 0), r, par),
-          src + off,
-          len,
-          hipMemcpyDeviceToDevice,
-          ss_->stream()));
-    }
-    launchWriteFlag(mesh_->peerFlag(dst, fDATA_ + r), seq, ss_->stream());
+    sends_.push_back(Chunk{dst, ++sendChunkSeq_[dst], src + off, len});
   }
+  enqueueReady();
 }
 
 void HipP2P::postRecv(
@@ -1792,41 +1752,103 @@ void HipP2P::postRecv(
   GA_HIP_CHECK(hipSetDevice(device_));
   GA_ENFORCE(src != ctx_->rank, "p2p recv from self");
   gateStreams(*gateRecvEv_, callerStream, {rs_->stream()});
-  char* dstPtr = static_cast<char*>(devPtr);
+  char* dst = static_cast<char*>(devPtr);
   const size_t nc = (bytes + chunkCap_ - 1) / chunkCap_;
   for (size_t c = 0; c < std::max<size_t>(nc, 1); c++) {
-    const uint64_t seq = ++recvChunkSeq_[src];
-    const int par = static_cast<int>(seq & 1);
-    launchWaitFlagGte(mesh_->flag(fDATA_ + src), seq, rs_->stream());
     const size_t off = c * chunkCap_;
     const size_t len = std::min(chunkCap_, bytes - std::min(bytes, off));
-    if (len > 0) {
-      GA_HIP_CHECK(hipMemcpyAsync(
-          dstPtr + off,
-          slotOf(mesh_->inbox(0), src, par),
-          len,
-          hipMemcpyDeviceToDevice,
-          rs_->stream()));
+    recvs_.push_back(Chunk{src, ++recvChunkSeq_[src], dst + off, len});
+  }
+  enqueueReady();
+}
+
+// Posted chunks go to their stream in order. Where ranks share a device no
+// wait is enqueued before its flag is there (see XgmiMesh::waitFlag), and
+// blocking in a post would keep the peer's sends from the receives that this
+// rank has yet to post: chunks that cannot go yet stay in the queue.
+void HipP2P::enqueueReady() {
+  const bool ahead = !mesh_->sharesDevice();
+  const int r = ctx_->rank;
+  for (bool moved = true; moved;) {
+    moved = false;
+    while (!sends_.empty()) {
+      const Chunk& c = sends_.front();
+      const int par = static_cast<int>(c.seq & 1);
+      if (c.seq > 2) {
+        // Same-parity slot reuse: dst consumed chunk seq-2.
+        if (!ahead && !mesh_->reached(fACK_ + c.peer, c.seq - 2)) {
+          break;
+        }
+        mesh_->waitFlag(fACK_ + c.peer, c.seq - 2, ss_->stream());
+      }
+      if (c.len > 0) {
+        GA_HIP_CHECK(hipMemcpyAsync(
+            slotOf(mesh_->peerInbox(c.peer, 0), r, par),
+            c.ptr,
+            c.len,
+            hipMemcpyDeviceToDevice,
+            ss_->stream()));
+      }
+      launchWriteFlag(
+          mesh_->peerFlag(c.peer, fDATA_ + r), c.seq, ss_->stream());
+      sends_.pop_front();
+      moved = true;
     }
-    launchWriteFlag(
-        mesh_->peerFlag(src, fACK_ + ctx_->rank), seq, rs_->stream());
+    while (!recvs_.empty()) {
+      const Chunk& c = recvs_.front();
+      const int par = static_cast<int>(c.seq & 1);
+      if (!ahead && !mesh_->reached(fDATA_ + c.peer, c.seq)) {
+        break;
+      }
+      mesh_->waitFlag(fDATA_ + c.peer, c.seq, rs_->stream());
+      if (c.len > 0) {
+        GA_HIP_CHECK(hipMemcpyAsync(
+            c.ptr,
+            slotOf(mesh_->inbox(0), c.peer, par),
+            c.len,
+            hipMemcpyDeviceToDevice,
+            rs_->stream()));
+      }
+      launchWriteFlag(
+          mesh_->peerFlag(c.peer, fACK_ + r), c.seq, rs_->stream());
+      recvs_.pop_front();
+      moved = true;
+    }
   }
 }
 
-void HipP2P::flushSends() {
+void HipP2P::flush(
+    std::deque<Chunk>& posted,
+    HipStream& stream,
+    const char* what) {
   GA_HIP_CHECK(hipSetDevice(device_));
+  const auto timeout = ctx_->getTimeout();
+  const auto deadline = std::chrono::steady_clock::now() + timeout;
+  for (;;) {
+    {
+      std::lock_guard<std::mutex> lock(mu_);
+      enqueueReady();
+      if (posted.empty()) {
+        break;
+      }
+    }
+    if (timeout.count() > 0 && std::chrono::steady_clock::now() > deadline) {
+      mesh_->fail(what);
+    }
+    std::this_thread::yield();
+  }
   HipEvent done(device_);
-  done.record(ss_->stream());
-  watchdogWait(done, *mesh_, ctx_->getTimeout(), "hip_p2p (sends)");
-  ss_->synchronize();
+  done.record(stream.stream());
+  watchdogWait(done, *mesh_, timeout, what);
+  stream.synchronize();
+}
+
+void HipP2P::flushSends() {
+  flush(sends_, *ss_, "hip_p2p (sends)");
 }
 
 void HipP2P::flushRecvs() {
-  GA_HIP_CHECK(hipSetDevice(device_));
-  HipEvent done(device_);
-  done.record(rs_->stream());
-  watchdogWait(done, *mesh_, ctx_->getTimeout(), "hip_p2p (recvs)");
-  rs_->synchronize();
+  flush(recvs_, *rs_, "hip_p2p (recvs)");
 }
 
 // ===========================================================================

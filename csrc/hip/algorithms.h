@@ -29,6 +29,7 @@
 #pragma once
 
 #include <array>
+#include <deque>
 #include <map>
 #include <memory>
 #include <mutex>
@@ -411,7 +412,8 @@ class HipP2P {
 
   // Enqueue a chunked device-to-device send/recv (async; returns once
   // enqueued). The caller's tensor must stay alive until the matching
-  // flush returns.
+  // flush returns. Where ranks of one process share the device, chunks past
+  // the two that a peer's inbox holds go on within later posts and flushes.
   void postSend(
       int dst,
       const void* devPtr,
@@ -427,6 +429,14 @@ class HipP2P {
   void flushRecvs();
 
  private:
+  struct Chunk {
+    int peer;
+    uint64_t seq;
+    char* ptr;
+    size_t len;
+  };
+  void enqueueReady(); // mu_ is held
+  void flush(std::deque<Chunk>& posted, HipStream& stream, const char* what);
   char* slotOf(char* inboxBase, int src, int par) {
     return inboxBase + (static_cast<size_t>(src) * 2 + par) * chunkCap_;
   }
@@ -445,6 +455,8 @@ class HipP2P {
   int fACK_; // [dst]: chunks dst consumed of my sends (monotonic)
   std::vector<uint64_t> sendChunkSeq_; // per dst lane
   std::vector<uint64_t> recvChunkSeq_; // per src lane
+  std::deque<Chunk> sends_; // posted, and not on their stream yet
+  std::deque<Chunk> recvs_;
   std::mutex mu_; // posts may come from several host threads
 };
 

@@ -57,6 +57,9 @@ void launchWriteFlag(uint64_t* addr, uint64_t val, hipStream_t stream);
 // makes peer SDMA-written data visible to later kernels on the stream).
 void launchWaitFlagGte(const uint64_t* addr, uint64_t val, hipStream_t stream);
 
+// Copies a flag's value to host memory (pinned), as the waits above see it.
+void launchReadFlag(const uint64_t* addr, uint64_t* host, hipStream_t stream);
+
 // Relative doorbells for hipGraph replay: target = *basePtr + offset,
 // evaluated at execution time (offset may be negative; non-positive
 // targets are no-ops). Always kernel-based (stream-op packets cannot be

@@ -287,6 +287,18 @@ __global__ __launch_bounds__(64) void waitFlagGteKernel(
   }
 }
 
+__global__ __launch_bounds__(64) void readFlagKernel(
+    const uint64_t* addr,
+    uint64_t* host) {
+  if (threadIdx.x == 0) {
+    __hip_atomic_store(
+        host,
+        __hip_atomic_load(addr, __ATOMIC_ACQUIRE, __HIP_MEMORY_SCOPE_SYSTEM),
+        __ATOMIC_RELEASE,
+        __HIP_MEMORY_SCOPE_SYSTEM);
+  }
+}
+
 // Relative doorbells for hipGraph replay: the flag target is
 // *basePtr + offset, read at EXECUTION time, so one captured graph can
 // replay with monotonically advancing sequence numbers (the host bumps
@@ -675,6 +687,15 @@ void launchWaitFlagGte(
   }
   hipLaunchKernelGGL(
       waitFlagGteKernel, dim3(1), dim3(64), 0, stream, addr, val);
+  GA_HIP_CHECK(hipGetLastError());
+}
+
+void launchReadFlag(
+    const uint64_t* addr,
+    uint64_t* host,
+    hipStream_t stream) {
+  hipLaunchKernelGGL(
+      readFlagKernel, dim3(1), dim3(64), 0, stream, addr, host);
   GA_HIP_CHECK(hipGetLastError());
 }
 

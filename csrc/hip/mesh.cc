@@ -2,11 +2,16 @@
 
 #include <unistd.h>
 
+#include <atomic>
+#include <chrono>
 #include <cstring>
+#include <string>
+#include <thread>
 
 #include "collectives/collectives.h"
 #include "common/logging.h"
 #include "common/utils.h"
+#include "hip/kernels.h"
 
 namespace glooamd {
 namespace hip {
@@ -85,6 +90,7 @@ XgmiMesh::XgmiMesh(
 
 void XgmiMesh::exchange() {
   const int P = ctx_->size;
+  sharesDevice_ = false;
   peerData_.assign(P, nullptr);
   peerFlags_.assign(P, nullptr);
   peerSameProcess_.assign(P, false);
@@ -124,6 +130,7 @@ void XgmiMesh::exchange() {
       peerData_[r] = reinterpret_cast<char*>(all[r].dataPtr);
       peerFlags_[r] = reinterpret_cast<uint64_t*>(all[r].flagsPtr);
       peerSameProcess_[r] = true;
+      sharesDevice_ = sharesDevice_ || all[r].device == device_;
     } else {
       void* p = nullptr;
       GA_HIP_CHECK(hipIpcOpenMemHandle(
@@ -224,6 +231,80 @@ int XgmiMesh::allocFlags(int count) {
   int base = nextFlag_;
   nextFlag_ += count;
   return base;
+}
+
+XgmiMesh::Reader::Reader(int device)
+    : stream(device), value(HipHostPointer<uint64_t>::alloc(1)) {}
+
+bool XgmiMesh::reached(int idx, uint64_t value) {
+  if (reader_ == nullptr) {
+    reader_ = std::make_unique<Reader>(device_);
+    seen_.assign(kNumFlags, 0);
+  }
+  if (seen_[idx] >= value) {
+    return true;
+  }
+  launchReadFlag(flag(idx), *reader_->value, reader_->stream.stream());
+  const auto timeout = ctx_->getTimeout();
+  const auto deadline = std::chrono::steady_clock::now() + timeout;
+  for (;;) {
+    const hipError_t e = hipStreamQuery(reader_->stream.stream());
+    if (e == hipSuccess) {
+      break;
+    }
+    if (e != hipErrorNotReady) {
+      GA_HIP_CHECK(e);
+    }
+    (void)hipGetLastError(); // not ready is no error
+    if (timeout.count() > 0 && std::chrono::steady_clock::now() > deadline) {
+      (void)reader_.release(); // the kernel may still write there
+      fail("reading a flag");
+    }
+    std::this_thread::yield();
+  }
+  seen_[idx] = **reader_->value;
+  return seen_[idx] >= value;
+}
+
+void XgmiMesh::waitFlag(int idx, uint64_t value, hipStream_t stream) {
+  if (sharesDevice_) {
+    const auto timeout = ctx_->getTimeout();
+    const auto deadline = std::chrono::steady_clock::now() + timeout;
+    while (!reached(idx, value)) {
+      if (timeout.count() > 0 &&
+          std::chrono::steady_clock::now() > deadline) {
+        fail("waiting for a peer's flag");
+      }
+      std::this_thread::yield();
+    }
+  }
+  // Where the host has waited, this passes at once, and orders what follows
+  // behind the peer's data.
+  launchWaitFlagGte(flag(idx), value, stream);
+}
+
+void XgmiMesh::fail(const char* what) {
+  std::string flags;
+  if (getEnvFlag("GLOO_AMD_FLAG_DEBUG")) {
+    for (uint64_t v : readFlags(16)) {
+      flags += " " + std::to_string(v);
+    }
+  }
+  poisonFlags();
+  // Bounded drain: a wedged hardware queue can make hipDeviceSynchronize hang
+  // forever; give it a few seconds on a helper thread, then fail fast (a
+  // leaked sync thread on a broken device is acceptable in the fail-fast model
+  // — the throw is what keeps the job from hanging).
+  auto done = std::make_shared<std::atomic<bool>>(false);
+  std::thread([done] {
+    (void)hipDeviceSynchronize();
+    done->store(true);
+  }).detach();
+  const auto dl = std::chrono::steady_clock::now() + std::chrono::seconds(8);
+  while (!done->load() && std::chrono::steady_clock::now() < dl) {
+    std::this_thread::sleep_for(std::chrono::milliseconds(10));
+  }
+  GA_THROW_IO("hip collective timed out in ", what, " flags:", flags);
 }
 
 void XgmiMesh::poisonFlags() {

@@ -11,7 +11,8 @@
 // The host only enqueues: the entire ring/halving-doubling schedule runs
 // on two HIP streams with GPU-side flag waits, so per-step host latency
 // (the reference's waitRecv/copyAsync round trips, cuda_allreduce_ring_
-// chunked.cc:130-273) disappears from the critical path.
+// chunked.cc:130-273) disappears from the critical path. (Ranks of one
+// process that share a GPU wait on the host: see waitFlag.)
 //
 // Construction is collective over a connected glooamd::Context: IPC
 // handles travel over the context's TCP pairs (v2 allgather).
@@ -77,6 +78,27 @@ class XgmiMesh {
   // allocation identical on every rank.
   int allocFlags(int count);
 
+  // Another rank of this process uses the same GPU.
+  bool sharesDevice() const {
+    return sharesDevice_;
+  }
+  // Work on `stream` behind this goes on once flag idx is at `value` or
+  // beyond. One rank of a process on a device: the device waits. All that the
+  // flag depends on is then other devices' or processes' work, or stands before
+  // the wait in the order in which this rank enqueues, and a collective could
+  // do all of it in that order, so its streams may share hardware queues.
+  // Several ranks: their streams share hardware queues with one another, and a
+  // wait at a queue's head can hold up the very work that it waits for. The
+  // host waits, and enqueues nothing that is not ready: no packet depends on
+  // one behind it, whichever queue it is in.
+  void waitFlag(int idx, uint64_t value, hipStream_t stream);
+  // Whether flag idx has come that far. Ranks that share a device only.
+  bool reached(int idx, uint64_t value);
+
+  // Gives a collective up: releases the waits, drains what can be drained
+  // within seconds and throws.
+  [[noreturn]] void fail(const char* what);
+
   // Host-side poison: release every local GPU-side flag wait (used by the
   // run() watchdog on timeout so streams can drain before throwing).
   void poisonFlags();
@@ -100,6 +122,17 @@ class XgmiMesh {
   std::vector<uint64_t*> peerFlags_;
   std::vector<bool> peerSameProcess_;
   int nextFlag_{0};
+
+  bool sharesDevice_{false};
+  // How the host reads flags, if it has to: by a kernel, which sees them as
+  // the device's own waits do.
+  struct Reader {
+    explicit Reader(int device);
+    HipStream stream;
+    HipHostPointer<uint64_t> value;
+  };
+  std::unique_ptr<Reader> reader_;
+  std::vector<uint64_t> seen_; // flags only grow
 };
 
 } // namespace hip
