@@ -71,8 +71,9 @@ class HipStream {
 // process+device; streams beyond that SHARE a queue, and a flag wait
 // then head-of-line-blocks whatever shares its queue. XgmiMesh::waitFlag
 // says why that does not deadlock; it costs overlap. Capping each
-// communicator at 8 pooled streams (index 0 = high priority) keeps every
-// stream on its own hardware queue. Pool key: one per (communicator, device) —
+// communicator at 8 pooled streams (index 0 = high priority, of another set
+// of queues: docs/stability.md) keeps every stream on its own hardware
+// queue. Pool key: one per (communicator, device) —
 // different algorithm objects of one communicator intentionally reuse
 // the same streams (collectives on a communicator are serialized).
 constexpr int kStreamPoolSize = 8;
