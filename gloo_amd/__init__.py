@@ -7,6 +7,8 @@ collectives over xGMI (hipIpcMemHandle peer transport) for GPU tensors.
 """
 
 import os as _os
+import sys as _sys
+import warnings as _warnings
 
 # 8 hardware queues per process so each pooled stream owns one (the
 # ROCm default of 4 would multiplex streams onto shared queues, where a
@@ -19,8 +21,16 @@ def _need_queues(least=8):
         have = int(_os.environ.get("GPU_MAX_HW_QUEUES", "0"))
     except ValueError:
         have = 0
-    if have < least:
-        _os.environ["GPU_MAX_HW_QUEUES"] = str(least)
+    if have >= least:
+        return
+    torch = _sys.modules.get("torch")
+    if torch is not None and torch.cuda.is_initialized():
+        _warnings.warn(
+            f"gloo_amd: the GPU was used before the import, with "
+            f"{have or 4} hardware queues: streams of its device collectives "
+            f"will share them, which costs overlap. Import gloo_amd first, or "
+            f"set GPU_MAX_HW_QUEUES={least}.", RuntimeWarning, stacklevel=3)
+    _os.environ["GPU_MAX_HW_QUEUES"] = str(least)
 
 
 _need_queues()
