@@ -1655,16 +1655,28 @@ int64_t tilesOf(T, const ProductShape& p, bool grouped) {
 // How many times 16 rows fewRowsKernel takes at a time, 0 where tiles are
 // better. Measured by 8192 x 4096, this kernel and tiles in us, for bf16
 // results: 1 row 7 / 10.4, 4 rows 8.2 / 10.2, 16 rows 10.8 / 10.6; for fp32
-// (and fp16) ones, whose tiles take longer: 16 rows 13.6 / 15.2, 32 rows 18.1 / 15.4 (by
-// 4096 x 4096 10.4 / 15.5). 8 rows for 8 of 16 experts of 1024 x 4096 8.5 /
-// 11.9, of 32 of 4096 x 2048 14.9 / 13.8, 16 rows of 16 experts 19.6 / 13.4;
-// fp32 4 rows 8.2 / 16.5 and 11.3 / 10.9, 8 rows 12.6 / 16.5 and 18.8 / 15.7.
+// (and fp16) ones, whose tiles take longer: 16 rows 13.6 / 15.2, 32 rows 18.1 /
+// 15.4 (by 4096 x 4096 10.4 / 15.5).
+// Of several experts each has workgroups for all of its columns, without rows
+// too, and with many of them those cost what the others save: from some 4096 on
+// (64 experts with 1024 columns, 16 with 4096), for one or two rows from 8192.
+// 4 rows, bf16 and fp32: 32 experts of 1024 x 4096 8.3 / 8.4 and 8.6 / 15.3, 64
+// of them 9.9 / 8.7 and 11.2 / 15.7, 128 of them 12.0 / 9.8 and 17.7 / 16.7; 16
+// experts of 4096 x 2048 8.1 / 8.2 and 9.5 / 10.5, 32 of them 9.7 / 8.1 and
+// 11.2 / 10.4. 1 row: 32 of those 5.1 / 6.4 and 5.7 / 9.9, 64 of them 8.0 / 6.8
+// and 8.6 / 10.1. 8 rows: bf16, 8 experts of 1024 x 4096 7.6 / 8.5, 16 of 4096 x
+// 2048 13.7 / 13.7; fp32, 32 of 4096 x 2048 18.8 / 15.7.
+constexpr int64_t kFewWorkgroups = 4096;
+
 int fewRows(const ProductShape& p, bool grouped, bool exact) {
   if (!p.aWhole || !p.bWhole) {
     return 0;
   }
   if (grouped) {
-    return p.m <= (exact ? 4 : 8) ? 1 : 0;
+    const int64_t most = p.m <= 2 ? 2 * kFewWorkgroups : kFewWorkgroups;
+    return p.m <= (exact ? 4 : 8) && p.experts * ((p.n + 15) / 16) <= most
+        ? 1
+        : 0;
   }
   if (exact) {
     return p.m <= 16 ? 1 : p.m <= 32 ? 2 : 0;

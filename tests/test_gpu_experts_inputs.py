@@ -252,6 +252,33 @@ def test_products_repeat_themselves(out):
             same(run, runs[0])
 
 
+@pytest.mark.parametrize("out", [torch.float32, torch.float16,
+                                 torch.bfloat16])
+@pytest.mark.parametrize("experts,n", [(1, 72), (3, 16), (16, 1030),
+                                       (16, 4096), (70, 1024), (70, 20)])
+@pytest.mark.parametrize("inner", [16, 208, 1024, 4224])
+def test_few_rows_of_experts(experts, n, inner, out):
+    """Whole numbers, whose sums are exact, on either side of where tiles take
+    over, with rows before the first expert's and behind the last one's."""
+    gen = torch.Generator().manual_seed(experts + n + inner)
+    b = torch.randint(-3, 4, (experts, n, inner), generator=gen).float()
+    qb = b.cuda().to(F8)
+    sb = torch.ones(experts, nb(n), nb(inner)).to(E8).cuda()
+    for rows in range(1, 10):
+        a = torch.randint(-3, 4, (rows, inner), generator=gen).float()
+        at = torch.randint(0, rows + 1, (experts + 1,), generator=gen)
+        at = torch.sort(at).values
+        sa = torch.ones(rows, nb(inner)).to(E8).cuda()
+        got = ex.fp8_matmul(a.cuda().to(F8), sa, qb, sb,
+                            offsets=at.int().cuda(), dtype=out).cpu()
+        want = torch.zeros(rows, n)
+        for e in range(experts):
+            part = slice(int(at[e]), int(at[e + 1]))
+            if part.start < part.stop:
+                want[part] = a[part] @ b[e].t()
+        assert torch.equal(got, want.to(out)), rows
+
+
 # ---------------------------------------------------------------- what is kept
 
 
