@@ -1,5 +1,6 @@
-// Python bindings of the expert-parallel operators and 8-bit products
-// (device pointers; gloo_amd/experts.py checks tensors and calls them).
+// Python bindings of the expert-parallel operators' and 8-bit products'
+// launches, by device pointers, for callers without torch (gloo_amd/experts.py
+// goes through csrc/torch/operators.cc), and the launches as one pointer.
 #pragma once
 
 #include <pybind11/pybind11.h>

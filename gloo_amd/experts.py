@@ -427,9 +427,12 @@ class ExpertExchange:
 
     Rank r of `group` (a "glooamd" process group, the default one if None)
     holds experts r * E / size to (r + 1) * E / size - 1. Each rank packs its
-    tokens by expert, the counts travel as a small alltoall of host tensors
-    (so that dispatch waits for the GPU once), the rows as one alltoall with
-    split sizes, and what arrives from the ranks is packed by expert again.
+    tokens by expert, the counts travel as a small alltoall of host tensors,
+    the rows as one alltoall with split sizes, and what arrives from the ranks
+    is packed by expert again. An alltoall with split sizes goes through host
+    memory and the CPU transport in this backend: dispatch, combine and their
+    backward passes wait for the GPU and copy their rows there and back (a
+    group of one rank does not).
     All ranks call both methods, ranks without tokens too, with rows of one
     length and type. With 16- or 32-bit rows the whole way is differentiable,
     and all ranks run its backward pass; with `fp8` the rows and their scales
