@@ -1,8 +1,7 @@
 """Expert operators on inputs that are not plain tensors, and on values where
 sums and exponentials lose what matters.
 
-Tolerances count roundings, as in test_gpu_experts.py, and its tests' names
-and order hold here too: these run behind test_gpu.py."""
+Tolerances count roundings, as in test_gpu_experts.py."""
 import pytest
 
 import gloo_amd as ga
