@@ -1831,9 +1831,13 @@ void HipP2P::flush(
       if (posted.empty()) {
         break;
       }
-    }
-    if (timeout.count() > 0 && std::chrono::steady_clock::now() > deadline) {
-      mesh_->fail(what);
+      if (timeout.count() > 0 &&
+          std::chrono::steady_clock::now() > deadline) {
+        // Giving up lets every wait pass, and callers free their tensors.
+        sends_.clear();
+        recvs_.clear();
+        mesh_->fail(what);
+      }
     }
     std::this_thread::yield();
   }

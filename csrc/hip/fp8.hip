@@ -1641,9 +1641,10 @@ constexpr int64_t kEnough = 192;
 // 2048 (about eight steps): 367 us against 414 with the large tile for fp32
 // results, 250 / 290 for bf16; 4 experts, some 32 steps, are even.
 constexpr int kShort = 32;
-// So are products with fp32 or fp16 results and a short inner dimension: 8192 x 4096 x
-// 512 48 us against 50, 8741 x 4096 x 512 of 8 experts 62 / 72, 16384 x 2048 x
-// 1024 of 16 84 / 95, 8192 x 8192 x 2048 244 / 255; from there on even.
+// So are products with fp32 or fp16 results and a short inner dimension: 8192 x
+// 4096 x 512 48 us against 50, 8741 x 4096 x 512 of 8 experts 62 / 72, 16384 x
+// 2048 x 1024 of 16 84 / 95, 8192 x 8192 x 2048 244 / 255 (279 on inputs that
+// alternate); from there on even.
 constexpr int kShortInner = 16;
 
 // Tiles of rows, at most: every expert's last one may be a part of one, and

@@ -145,3 +145,22 @@ def test_a_rank_that_does_not_come_is_given_up():
         ga.barrier(ctx, tag=821)
 
     ranks(2, fn)
+
+
+def test_sends_that_nobody_receives_are_given_up():
+    """And what was still to go is dropped: the tensor may be freed."""
+    from gloo_amd import IoError
+
+    def fn(ctx, rank):
+        engine = ga._C.HipP2P(ctx, 0)
+        ga.barrier(ctx, tag=830)
+        if rank == 0:
+            ctx.set_timeout(500)
+            x = torch.ones(6_000_000, device="cuda")
+            engine.post_send(1, x.data_ptr(), x.numel() * 4, stream())
+            with pytest.raises(IoError, match="timed out"):
+                engine.flush_sends()
+            engine.flush_sends()  # nothing is left
+        ga.barrier(ctx, tag=831)
+
+    ranks(2, fn)
