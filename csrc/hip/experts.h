@@ -82,7 +82,7 @@ void launchExpertPack(
     hipStream_t stream);
 // The same in e4m3 with a power of two (e8m0) for each 128 elements. q's
 // rows are qStride bytes apart, a multiple of 16 that is at least hidden;
-// the bytes between are zeros. scales: [tokens * k, ceil(hidden / 128)].
+// the bytes between are zeros (NaN where the last block's are). scales: [tokens * k, ceil(hidden / 128)].
 void launchExpertPackFp8(
     const ExpertRowsArgs& args,
     const void* x,

@@ -20,7 +20,8 @@ constexpr int kFp8Block = 128; // elements along a row that share a scale
 
 // q[r, c] = e4m3(x[r, c] / 2^e) and the scales' e of each 1 x 128 block
 // (scales [rows, ceil(cols / 128)]). x has any strides. q's rows are qStride
-// bytes apart, a multiple of 16; the bytes between are zeros.
+// bytes apart, a multiple of 16; the bytes between are zeros (NaN where the
+// last block's are).
 void launchQuantizeFp8(
     const void* x,
     int64_t rowStride,
